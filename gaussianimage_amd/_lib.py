@@ -35,6 +35,8 @@ PROBE = {"project": 1, "raster_fwd": 2, "raster_bwd": 3, "gather": 4, "fit_raste
          "fit_tail": 6}
 
 BLOCK = 16
+ADAMW_BLOCK = 256         # GI2D_ADAMW_BLOCK
+ADAMW_SCALARS_BYTES = 64  # GI2D_ADAMW_SCALARS_BYTES
 MAX_COLOR_SETS = 3  # GI2D_MAX_COLOR_SETS
 MAX_VQ_LAYERS = 8   # GI2D_MAX_VQ_LAYERS
 NOALLOC_MAX_TILES = 34816        # GI2D_NOALLOC_MAX_TILES
@@ -47,6 +49,21 @@ class AdanHyper(ctypes.Structure):
                 ("beta3", ctypes.c_double), ("eps", ctypes.c_double),
                 ("weight_decay", ctypes.c_double), ("no_prox", ctypes.c_int),
                 ("step", ctypes.c_int)]
+
+
+class AdamWTensor(ctypes.Structure):
+    """Mirror of ``gi2d_adamw_tensor``."""
+    _fields_ = [(n, ctypes.c_void_p) for n in
+                ("param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale",
+                 "master")] + \
+               [("numel", ctypes.c_int64), ("param_type", ctypes.c_int), ("grad_type", ctypes.c_int)]
+
+
+class AdamWHyper(ctypes.Structure):
+    """Mirror of ``gi2d_adamw_hyper``."""
+    _fields_ = [(n, ctypes.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay")] + \
+               [("step", ctypes.c_int64), ("seed", ctypes.c_uint32), ("state_bits", ctypes.c_int)] + \
+               [(n, ctypes.c_void_p) for n in ("step_dev", "lr_dev", "scalars_dev")]
 
 
 class Codec(ctypes.Structure):
@@ -129,6 +146,10 @@ SIGNATURES = {
                                     _vp, _vp, _vp, _vp, _vp, _vp, ctypes.POINTER(AdanHyper), _vp]),
     "gi2d_adan_step": (_i, [_i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.POINTER(AdanHyper), _vp,
                             _vp]),
+    "gi2d_adamw_step": (_i, [_i, ctypes.POINTER(AdamWTensor), ctypes.POINTER(AdamWHyper), _vp,
+                             _vp]),
+    "gi2d_grad_norm_workspace": (_i64, [_i]),
+    "gi2d_grad_norm": (_i, [_i, _vp, _vp, _vp, ctypes.c_double, _vp, _vp, _vp]),
     "gi2d_rasterize_sum_bwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _convp, _vp, _vp,
                                     _vp, _vp, _vp, _vp]),
 }

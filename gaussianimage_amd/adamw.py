@@ -1,0 +1,423 @@
+"""AdamW over many tensors at once, with states in 32 bits or in 8, and the norm of all gradients
+with its clip coefficient -- beside ``adan.Adan`` for fits and trainings that want Adam's update.
+
+``AdamW`` is the optimizer; ``adamw_step``, ``adamw_step_8bit`` and ``grad_norm`` are the calls it
+makes, for programs that keep their states themselves.  One launch steps up to 64 tensors (48 with
+8-bit states) of the same types.  GPU only, like the rest of the package: tensors on the CPU raise.
+"""
+import ctypes
+
+import torch
+from torch.optim.optimizer import Optimizer
+
+from . import _lib, ops
+from ._lib import ADAMW_BLOCK, check, lib
+
+__all__ = ["AdamW", "adamw_step", "adamw_step_8bit", "grad_norm", "zero_state_8bit"]
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_CODES = torch.float8_e4m3fn
+
+
+# ------------------------------------------------------------------------------ the operators
+
+def grad_norm(grads, max_norm=None):
+    """2-norm of all ``grads`` together, and ``min(1, max_norm / (norm + 1e-6))``: two float32
+    scalars on the device (``(norm, None)`` without ``max_norm``).  Float32, bfloat16 and float16
+    gradients may be mixed.  Squares are summed in double and in a fixed order."""
+    if max_norm is not None and not max_norm >= 0.0:
+        raise ValueError(f"grad_norm: max_norm must be >= 0, got {max_norm}")
+    limit = float("inf") if max_norm is None else float(max_norm)
+    norm, coef = (ops._C if ops._USE_C else _ctypes_binding).grad_norm(grads, limit)
+    return norm, (None if max_norm is None else coef)
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.9, 0.999),
+               eps=1e-8, weight_decay=1e-2, masters=None, clip=None):
+    """One AdamW step (decoupled weight decay) of every tensor, in place, with float32 states:
+
+        g = clip * grad,  m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2
+        p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+
+    ``params`` and ``grads`` are float32, bfloat16 or float16, each tensor its own; arithmetic is
+    float32, and a half parameter is rounded to nearest at the end.  ``masters`` (or single entries
+    of it) may hold float32 copies of half parameters: then the copy is read and updated and the
+    parameter is its rounding.  ``step`` counts from 1; it may be an int64 tensor and ``lr`` a
+    float32 tensor of one element on the device, both read when the step runs (for captured
+    steps).  ``clip``: a device scalar, ``grad_norm``'s second result.  Gradients are not written.
+
+    Every tensor must be dense, and a parameter's gradient and states laid out as it is.
+    """
+    _check_hyper("adamw_step", lr, betas, eps, weight_decay, 0)
+    (ops._C if ops._USE_C else _ctypes_binding).adamw_step(
+        "adamw_step", 32, params, grads, exp_avgs, exp_avg_sqs, None, None, masters, step, lr,
+        betas[0], betas[1], eps, weight_decay, 0, clip)
+
+
+def adamw_step_8bit(params, grads, exp_avgs, exp_avg_scales, exp_avg_rms, exp_avg_rms_scales, *,
+                    step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, seed=0,
+                    masters=None, clip=None):
+    """``adamw_step`` with states of 8 bits: ``exp_avgs`` holds m and ``exp_avg_rms`` sqrt(v) as
+    float8_e4m3fn codes laid out as the parameter, each times the float32 scale (a power of two) of
+    its block of 256 consecutive elements in memory.  ``zero_state_8bit`` makes the four tensors of
+    a parameter.
+
+    The parameter is updated with m and v before they are rounded.  The codes are rounded at random
+    with the mean kept -- v moves by 0.1 % a step where neighbouring codes are 6 to 12 % apart --
+    by a hash of (``seed``, ``step``, block, element), so that the same call gives the same bits.
+    A sqrt(v) that is not zero never becomes zero; infinities and NaN become the NaN code.
+    """
+    _check_hyper("adamw_step_8bit", lr, betas, eps, weight_decay, seed)
+    (ops._C if ops._USE_C else _ctypes_binding).adamw_step(
+        "adamw_step_8bit", 8, params, grads, exp_avgs, exp_avg_rms, exp_avg_scales,
+        exp_avg_rms_scales, masters, step, lr, betas[0], betas[1], eps, weight_decay, seed, clip)
+
+
+def zero_state_8bit(param):
+    """``(exp_avg, exp_avg_scale, exp_avg_rms, exp_avg_rms_scale)`` of a parameter that has not
+    been stepped yet."""
+    blocks = (param.numel() + ADAMW_BLOCK - 1) // ADAMW_BLOCK
+
+    def codes():
+        return torch.zeros_like(param, dtype=torch.uint8, requires_grad=False).view(_CODES)
+
+    def scales():
+        return torch.zeros(blocks, dtype=torch.float32, device=param.device)
+
+    return codes(), scales(), codes(), scales()
+
+
+def _check_hyper(op, lr, betas, eps, weight_decay, seed):
+    if not torch.is_tensor(lr) and not lr >= 0.0:
+        raise ValueError(f"{op}: lr must be >= 0, got {lr}")
+    if not eps >= 0.0:
+        raise ValueError(f"{op}: eps must be >= 0, got {eps}")
+    if not weight_decay >= 0.0:
+        raise ValueError(f"{op}: weight_decay must be >= 0, got {weight_decay}")
+    if len(betas) != 2 or not all(0.0 <= b < 1.0 for b in betas):
+        raise ValueError(f"{op}: two betas in [0, 1) expected, got {betas}")
+    if not 0 <= seed < 2 ** 32:
+        raise ValueError(f"{op}: seed must be in [0, 2^32), got {seed}")
+
+
+# ------------------------------------------------------------------------------ over ctypes
+
+class _ctypes_binding:
+    """The two calls of the compiled binding, over ctypes (more host time per call)."""
+
+    @staticmethod
+    def _dense(t):
+        if t.is_contiguous():
+            return True
+        expect = 1  # strides in rising order multiply up without gaps
+        for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
+            if stride != expect:
+                return False
+            expect *= size
+        return True
+
+    @staticmethod
+    def _device_scalar(op, name, t, dtype, device):
+        if t.numel() != 1 or t.dtype != dtype or t.device != device:
+            raise ValueError(f"{op}: {name} must be a {dtype} tensor of one element on the "
+                             "parameters' device")
+        return t.data_ptr()
+
+    @classmethod
+    def adamw_step(cls, op, bits, params, grads, exp_avgs, exp_avg_sqs, scales, sq_scales, masters,
+                   step, lr, beta1, beta2, eps, weight_decay, seed, clip):
+        names = {"params": params, "grads": grads, "exp_avgs": exp_avgs,
+                 "exp_avg_rms" if bits == 8 else "exp_avg_sqs": exp_avg_sqs}
+        if bits == 8:
+            names["exp_avg_scales"], names["exp_avg_rms_scales"] = scales, sq_scales
+        if masters is not None:
+            names["masters"] = masters
+        n = len(params)
+        for name, ts in names.items():
+            if len(ts) != n:
+                raise ValueError(f"{op}: {name} has {len(ts)} entries, params has {n}")
+            for i, t in enumerate(ts):
+                if not torch.is_tensor(t) and not (name == "masters" and t is None):
+                    raise TypeError(f"{name}[{i}] is not a tensor")
+        if n == 0:
+            return
+        device = params[0].device
+        state_type = _CODES if bits == 8 else torch.float32
+        table = (_lib.AdamWTensor * n)()
+        seen = set()
+        for i in range(n):
+            p, t = params[i], table[i]
+            w = masters[i] if masters is not None else None
+
+            def refuse(name, what):
+                raise ValueError(f"{op}: {name}[{i}] {what}")
+
+            def laid_out(x):
+                return x.shape == p.shape and (x.is_contiguous() if p.is_contiguous()
+                                               else x.stride() == p.stride())
+
+            for x in (p, grads[i], exp_avgs[i], exp_avg_sqs[i], w):
+                if x is not None:
+                    if x.layout != torch.strided:
+                        refuse("params", "or what belongs to it is not strided")
+                    if x.device != device:
+                        refuse("params", "or what belongs to it is on another device")
+            for name, x in (("params", p), ("grads", grads[i])):
+                if x.dtype not in _TYPES:
+                    refuse(name, "must be float32, bfloat16 or float16")
+            if not cls._dense(p):
+                refuse("params", "has gaps or overlaps in memory")
+            if not laid_out(grads[i]):
+                refuse("grads", "is not laid out as its parameter")
+            for name, x in list(names.items())[2:4]:
+                if x[i].dtype != state_type or not laid_out(x[i]):
+                    refuse(name, f"must be a {str(state_type)[6:]} tensor laid out as its parameter")
+            t.numel = p.numel()
+            if t.numel > 2 ** 34:
+                refuse("params", "has more than 2^34 elements")
+            t.param_type, t.grad_type = _TYPES[p.dtype], _TYPES[grads[i].dtype]
+            t.param, t.grad = ops._ptr(p), ops._ptr(grads[i])
+            t.exp_avg, t.exp_avg_sq = ops._ptr(exp_avgs[i]), ops._ptr(exp_avg_sqs[i])
+            out = [p, exp_avgs[i], exp_avg_sqs[i]]
+            if w is not None:
+                if p.dtype == torch.float32:
+                    refuse("masters", "belongs to a float32 parameter")
+                if w.dtype != torch.float32 or not laid_out(w):
+                    refuse("masters", "must be a float32 tensor laid out as its parameter")
+                t.master = ops._ptr(w)
+                out.append(w)
+            if t.numel:
+                for x in out:
+                    if x.data_ptr() in seen:
+                        refuse("params", "or its state appears twice")
+                    seen.add(x.data_ptr())
+            if bits == 8:
+                blocks = (t.numel + ADAMW_BLOCK - 1) // ADAMW_BLOCK
+                for name, x in list(names.items())[4:6]:
+                    if x[i].dtype != torch.float32 or x[i].numel() != blocks or \
+                            not x[i].is_contiguous() or x[i].device != device:
+                        refuse(name, "must be a contiguous float32 tensor with one element for 256 "
+                               "of the parameter's, on its device")
+                t.exp_avg_scale, t.exp_avg_sq_scale = ops._ptr(scales[i]), ops._ptr(sq_scales[i])
+        ops._need_cuda(op, params[0])
+        h = _lib.AdamWHyper(beta1=beta1, beta2=beta2, eps=eps, weight_decay=weight_decay, seed=seed,
+                            state_bits=bits, step=1)
+        with torch.cuda.device(device):
+            if torch.is_tensor(step):
+                h.step_dev = cls._device_scalar(op, "step", step, torch.int64, device)
+            else:
+                h.step = int(step)
+            if h.step < 1:
+                raise ValueError(f"{op}: step counts from 1")
+            if torch.is_tensor(lr):
+                h.lr_dev = cls._device_scalar(op, "lr", lr, torch.float32, device)
+            else:
+                h.lr = float(lr)
+            if h.step_dev or h.lr_dev:
+                work = torch.empty(_lib.ADAMW_SCALARS_BYTES, dtype=torch.uint8, device=device)
+                h.scalars_dev = work.data_ptr()
+            if clip is not None:
+                if not torch.is_tensor(clip):
+                    raise TypeError(f"{op}: clip must be a tensor (grad_norm's second result)")
+                clip = cls._device_scalar(op, "clip", clip, torch.float32, device)
+            check(lib.gi2d_adamw_step(n, table, ctypes.byref(h), clip, ops._stream(device)),
+                  "gi2d_adamw_step")
+        for name, ts in names.items():
+            if name != "grads":
+                for x in ts:
+                    if x is not None and not x.is_inference():
+                        torch.autograd.graph.increment_version(x)
+
+    @classmethod
+    def grad_norm(cls, grads, max_norm):
+        n = len(grads)
+        if n == 0:
+            raise ValueError("grad_norm: no gradients")
+        for i, g in enumerate(grads):
+            if not torch.is_tensor(g):
+                raise TypeError(f"grads[{i}] is not a tensor")
+            if g.layout != torch.strided:
+                raise ValueError(f"grad_norm: grads[{i}] is not strided")
+            if g.device != grads[0].device:
+                raise ValueError(f"grad_norm: grads[{i}] is on another device")
+            if g.dtype not in _TYPES:
+                raise ValueError(f"grad_norm: grads[{i}] must be float32, bfloat16 or float16")
+            if not cls._dense(g):
+                raise ValueError(f"grad_norm: grads[{i}] has gaps or overlaps in memory")
+            if g.numel() > 2 ** 34:
+                raise ValueError(f"grad_norm: grads[{i}] has more than 2^34 elements")
+        ops._need_cuda("grad_norm", grads[0])
+        device = grads[0].device
+        with torch.cuda.device(device):
+            work = torch.empty(lib.gi2d_grad_norm_workspace(n), dtype=torch.uint8, device=device)
+            out = torch.empty(2, dtype=torch.float32, device=device)
+            check(lib.gi2d_grad_norm(n, (ctypes.c_void_p * n)(*[ops._ptr(g) for g in grads]),
+                                     (ctypes.c_int64 * n)(*[g.numel() for g in grads]),
+                                     (ctypes.c_int * n)(*[_TYPES[g.dtype] for g in grads]),
+                                     max_norm, work.data_ptr(), out.data_ptr(),
+                                     ops._stream(device)), "gi2d_grad_norm")
+        return out[0], out[1]
+
+
+# ------------------------------------------------------------------------------ the optimizer
+
+class AdamW(Optimizer):
+    """AdamW with fused steps.
+
+    ``state_bits``: 32, or 8 for states of two bytes per element (see ``adamw_step_8bit``;
+    ``seed`` drives their rounding).  ``master_weights``: keep a float32 copy of every half
+    parameter and update that.  ``max_grad_norm`` > 0: all gradients together are scaled to at
+    most that norm as they are read (``p.grad`` itself stays as it is).
+
+    ``capturable=True`` keeps the step counts in device memory, so that ``step()`` may be captured
+    into a graph (after one step outside of it, which makes the states) and replayed; then ``lr``
+    may be a float32 tensor on the device that is changed between replays.  Parameters that have
+    been stepped together must then go on being stepped together.
+    """
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
+                 max_grad_norm=0.0, state_bits=32, master_weights=False, capturable=False, seed=0):
+        _check_hyper("AdamW", lr, betas, eps, weight_decay, seed)
+        if not max_grad_norm >= 0.0:
+            raise ValueError(f"AdamW: max_grad_norm must be >= 0, got {max_grad_norm}")
+        if state_bits not in (32, 8):
+            raise ValueError(f"AdamW: state_bits must be 32 or 8, got {state_bits}")
+        self.max_grad_norm, self.state_bits, self.seed = float(max_grad_norm), state_bits, seed
+        self.master_weights, self.capturable = bool(master_weights), bool(capturable)
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps,
+                                      weight_decay=weight_decay))
+
+    def _new_state(self, p, step):
+        state = {"step": step}
+        if self.state_bits == 8:
+            (state["exp_avg"], state["exp_avg_scale"], state["exp_avg_rms"],
+             state["exp_avg_rms_scale"]) = zero_state_8bit(p)
+        else:
+            state["exp_avg"] = torch.zeros_like(p, dtype=torch.float32)
+            state["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32)
+        if self.master_weights and p.dtype != torch.float32:
+            state["master"] = p.detach().to(torch.float32)
+        return state
+
+    def _gradient(self, p):
+        g = p.grad
+        if not p.is_cuda:
+            raise RuntimeError("gaussianimage_amd.AdamW steps parameters on an AMD GPU only "
+                               "(there is no CPU fallback)")
+        if g.layout != torch.strided:
+            raise RuntimeError("AdamW: sparse gradients are not supported")
+        if g.stride() != p.stride():  # (an order of its own, or broadcast)
+            g = torch.empty_like(p, dtype=g.dtype, requires_grad=False).copy_(g)
+        return g
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        capturing = torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
+        if capturing and not self.capturable:
+            raise RuntimeError("AdamW: only an optimizer made with capturable=True can be captured")
+        # what is stepped together: the same group, device and step count
+        calls, norm_grads, absent = {}, [], set()
+        for k, group in enumerate(self.param_groups):
+            fresh = {}  # device -> the count that new states share
+            for p in group["params"]:
+                state = self.state.get(p)
+                if p.grad is None:
+                    if state and self.capturable:
+                        absent.add(id(state["step"]))
+                    continue
+                g = self._gradient(p)
+                if not state:
+                    if capturing:
+                        raise RuntimeError("AdamW: run one step before capturing (a captured "
+                                           "step cannot make the states)")
+                    if self.capturable and p.device not in fresh:
+                        fresh[p.device] = torch.zeros(1, dtype=torch.int64, device=p.device)
+                    state = self.state[p] = self._new_state(
+                        p, fresh[p.device] if self.capturable else 0)
+                count = state["step"]
+                key = (k, p.device, id(count) if self.capturable else count)
+                call = calls.setdefault(key, (count, [], [], []))
+                call[1].append(p)
+                call[2].append(g)
+                call[3].append(state)
+                norm_grads.append(g)
+        if not calls:
+            return loss
+        if any(id(count) in absent for count, *_ in calls.values()) and self.capturable:
+            raise RuntimeError("AdamW(capturable=True): parameters that were stepped together "
+                               "must go on having gradients together")
+        clip = None
+        if self.max_grad_norm > 0:
+            clip = grad_norm(norm_grads, self.max_grad_norm)[1]
+        for number, ((k, _, _), (count, ps, gs, states)) in enumerate(calls.items()):
+            group = self.param_groups[k]
+            lr = group["lr"]
+            if torch.is_tensor(lr) and not lr.is_cuda:
+                lr = float(lr)
+            count += 1  # (in place for a tensor)
+            if not self.capturable:
+                for state in states:
+                    state["step"] = count
+            kw = dict(step=count, lr=lr, betas=group["betas"], eps=group["eps"],
+                      weight_decay=group["weight_decay"], clip=clip)
+            if self.master_weights:
+                kw["masters"] = [state.get("master") for state in states]
+
+            def column(name):
+                return [state[name] for state in states]
+
+            if self.state_bits == 8:
+                # (each call numbers its blocks from 0: another seed, other random words)
+                adamw_step_8bit(ps, gs, column("exp_avg"), column("exp_avg_scale"),
+                                column("exp_avg_rms"), column("exp_avg_rms_scale"),
+                                seed=(self.seed + 0x61C88647 * number) % 2 ** 32, **kw)
+            else:
+                adamw_step(ps, gs, column("exp_avg"), column("exp_avg_sq"), **kw)
+        return loss
+
+    def state_dict(self):
+        """As torch's, with the step counts as plain numbers (this synchronises when they are in
+        device memory)."""
+        sd = super().state_dict()
+        sd["state"] = {k: {**s, "step": int(s["step"])} for k, s in sd["state"].items()}
+        return sd
+
+    @torch.no_grad()
+    def load_state_dict(self, state_dict):
+        """Takes a ``state_dict()`` of an AdamW with the same ``state_bits``.  The states keep
+        their own types (torch would bring them to the parameters')."""
+        names = {"step", "exp_avg"} | ({"exp_avg_scale", "exp_avg_rms", "exp_avg_rms_scale"}
+                                       if self.state_bits == 8 else {"exp_avg_sq"})
+        for s in state_dict["state"].values():
+            if not names <= set(s) <= names | {"master"}:
+                raise ValueError("AdamW: the state_dict holds other states than state_bits="
+                                 f"{self.state_bits} needs: {sorted(s)}")
+        super().load_state_dict({**state_dict, "state": {}})
+        pairs = [(k, i, p) for k, (old, new) in enumerate(zip(state_dict["param_groups"],
+                                                              self.param_groups))
+                 for i, p in zip(old["params"], new["params"])]
+        counts = {}
+        for k, i, p in pairs:
+            if i not in state_dict["state"]:
+                continue
+            s = state_dict["state"][i]
+            state = self._new_state(p, int(s["step"]))
+            for name, t in state.items():
+                if name != "step" and name in s:
+                    if s[name].shape != t.shape or s[name].dtype != t.dtype:
+                        raise ValueError(f"AdamW: {name} of parameter {i} is {s[name].dtype} "
+                                         f"{tuple(s[name].shape)}, expected {t.dtype} "
+                                         f"{tuple(t.shape)}")
+                    t.view(torch.uint8 if t.dtype == _CODES else t.dtype).copy_(
+                        s[name].view(torch.uint8) if t.dtype == _CODES else s[name])
+            if self.capturable:
+                at = (k, p.device, state["step"])
+                if at not in counts:
+                    counts[at] = torch.full((1,), state["step"], dtype=torch.int64,
+                                            device=p.device)
+                state["step"] = counts[at]
+            self.state[p] = state

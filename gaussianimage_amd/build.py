@@ -12,7 +12,7 @@ from concurrent.futures import ThreadPoolExecutor
 _HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(_HERE, "csrc")
 SOURCES = ["lists.hip", "project.hip", "raster_fwd.hip", "raster_bwd.hip", "fit.hip",
-           "noalloc.hip"]
+           "noalloc.hip", "adamw.hip"]
 LIB = os.path.join(CSRC, "libgi2d.so")
 OBJ_DIR = os.path.join(CSRC, "_build")
 
@@ -78,6 +78,8 @@ def build_native(force=False, extra_flags=(), verbose=False, jobs=None):
 
 
 TORCH_OPS_SRC = os.path.join(CSRC, "torch_ops.cpp")
+TORCH_OPS_DEPS = [TORCH_OPS_SRC, os.path.join(CSRC, "torch_adamw.h"),
+                  os.path.join(os.path.dirname(_HERE), "include", "gi2d.h")]
 TORCH_OPS_LIB = os.path.join(_HERE, "_torch_ops.so")
 
 
@@ -85,15 +87,14 @@ def torch_ops_stale():
     if not os.path.exists(TORCH_OPS_LIB):
         return True
     t = os.path.getmtime(TORCH_OPS_LIB)
-    deps = [TORCH_OPS_SRC, os.path.join(os.path.dirname(_HERE), "include", "gi2d.h")]
-    return any(os.path.getmtime(d) > t for d in deps)
+    return any(os.path.getmtime(d) > t for d in TORCH_OPS_DEPS)
 
 
 def torch_ops_id():
     """Hash of what the compiled binding is built from, and the torch it is built against."""
     import torch
     h = hashlib.sha256()
-    for d in (TORCH_OPS_SRC, os.path.join(os.path.dirname(_HERE), "include", "gi2d.h")):
+    for d in TORCH_OPS_DEPS:
         h.update(open(d, "rb").read())
     return h.hexdigest()[:16] + "/torch-" + torch.__version__
 

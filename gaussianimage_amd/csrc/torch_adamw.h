@@ -1,0 +1,271 @@
+// torch_adamw.h -- gi2d_adamw_step and gi2d_grad_norm over Python lists of tensors (part of
+// torch_ops.cpp).  A list of some hundred small tensors is stepped in tens of microseconds on the
+// GPU, so the lists are read through the C API of lists, one pass, without a reference count per
+// tensor.  adamw.py holds the same calls over ctypes; both make the same checks.
+#pragma once
+
+namespace adamw {
+
+// A list or tuple of tensors (None allowed where `optional`).
+struct Tensors {
+    PyObject *fast = nullptr;
+    const char *name;
+    bool none;
+    Tensors(const py::object &o, const char *name_) : name(name_), none(o.is_none())
+    {
+        if (none) return;
+        fast = PySequence_Fast(o.ptr(), "a list of tensors expected");
+        if (fast == nullptr) throw py::error_already_set();
+    }
+    Tensors(const Tensors &) = delete;
+    Tensors &operator=(const Tensors &) = delete;
+    ~Tensors() { Py_XDECREF(fast); }
+    int64_t size() const { return none ? 0 : (int64_t)PySequence_Fast_GET_SIZE(fast); }
+    // nullptr: None, where that is allowed
+    const at::Tensor *at(int64_t i, bool optional = false) const
+    {
+        if (none) return nullptr;
+        PyObject *o = PySequence_Fast_GET_ITEM(fast, i);
+        if (optional && o == Py_None) return nullptr;
+        if (!THPVariable_Check(o))
+            throw py::type_error(std::string(name) + "[" + std::to_string(i) + "] is not a tensor");
+        return &THPVariable_Unpack(o);
+    }
+};
+
+[[noreturn]] inline void refuse(const char *op, const char *name, int64_t i, const char *what)
+{
+    throw py::value_error(std::string(op) + ": " + name + "[" + std::to_string(i) + "] " + what);
+}
+
+inline int element_type(const at::Tensor &t)
+{
+    switch (t.scalar_type()) {
+        case at::kFloat: return GI2D_F32;
+        case at::kBFloat16: return GI2D_BF16;
+        case at::kHalf: return GI2D_F16;
+        default: return -1;
+    }
+}
+
+inline void need_gpu(const char *op, const at::Tensor &t)
+{
+    if (t.is_cuda()) return;
+    std::ostringstream msg;
+    msg << op << ": this operator runs on an AMD GPU through the HIP library only; got a "
+        << t.device() << " tensor (there is no CPU fallback)";
+    throw std::runtime_error(msg.str());
+}
+
+// `t` holds its elements in the same places as `p` does, without gaps.
+inline bool same_layout(const at::Tensor &t, const at::Tensor &p, bool p_contiguous)
+{
+    if (t.sizes() != p.sizes()) return false;
+    return p_contiguous ? t.is_contiguous() : t.strides() == p.strides();
+}
+
+// Set of addresses that a call writes: a tensor given twice would be updated by two workgroups at
+// once.
+class Written {
+    std::vector<const void *> slots;
+    size_t mask;
+
+  public:
+    explicit Written(size_t n)
+    {
+        size_t size = 16;
+        while (size < 2 * n) size *= 2;
+        slots.assign(size, nullptr);
+        mask = size - 1;
+    }
+    bool add(const void *p)
+    {
+        size_t at = ((uintptr_t)p >> 4) * 0x9E3779B97F4A7C15ull >> 32 & mask;
+        for (; slots[at] != nullptr; at = (at + 1) & mask)
+            if (slots[at] == p) return false;
+        slots[at] = p;
+        return true;
+    }
+};
+
+inline void written(const at::Tensor &t)
+{
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+inline const at::Tensor *device_scalar(const char *op, const char *name, const py::object &o,
+                                       at::ScalarType type, const at::Device &device)
+{
+    const at::Tensor &t = THPVariable_Unpack(o.ptr());
+    if (t.numel() != 1 || t.scalar_type() != type || t.device() != device)
+        throw py::value_error(std::string(op) + ": " + name + " must be a " + at::toString(type) +
+                              " tensor of one element on the parameters' device");
+    return &t;
+}
+
+void step(const char *op, int bits, const py::object &params_, const py::object &grads_,
+          const py::object &m_, const py::object &v_, const py::object &sm_, const py::object &sv_,
+          const py::object &masters_, const py::object &step_, const py::object &lr_, double beta1,
+          double beta2, double eps, double weight_decay, uint32_t seed, const py::object &clip_)
+{
+    const Tensors params(params_, "params"), grads(grads_, "grads"), m(m_, "exp_avgs"),
+        v(v_, bits == 8 ? "exp_avg_rms" : "exp_avg_sqs"), sm(sm_, "exp_avg_scales"),
+        sv(sv_, "exp_avg_rms_scales"), masters(masters_, "masters");
+    const int64_t n = params.size();
+    const auto length = [&](const Tensors &t) {
+        if (t.size() != n)
+            throw py::value_error(std::string(op) + ": " + t.name + " has " +
+                                  std::to_string(t.size()) + " entries, params has " +
+                                  std::to_string(n));
+    };
+    length(grads);
+    length(m);
+    length(v);
+    if (bits == 8) {
+        length(sm);
+        length(sv);
+    }
+    if (!masters.none) length(masters);
+    if (n == 0) return;
+    const at::ScalarType state_type = bits == 8 ? at::kFloat8_e4m3fn : at::kFloat;
+    const char *state_what = bits == 8 ? "must be a float8_e4m3fn tensor laid out as its parameter"
+                                       : "must be a float32 tensor laid out as its parameter";
+    const at::Device device = params.at(0)->device();
+    std::vector<gi2d_adamw_tensor> ts((size_t)n);
+    Written seen((size_t)n * 4);
+    for (int64_t i = 0; i < n; ++i) {
+        const at::Tensor &p = *params.at(i), &g = *grads.at(i), &mi = *m.at(i), &vi = *v.at(i);
+        const at::Tensor *w = masters.at(i, true);
+        gi2d_adamw_tensor &t = ts[(size_t)i];
+        const at::Tensor *const all[5] = {&p, &g, &mi, &vi, w};
+        for (const at::Tensor *x : all)
+            if (x != nullptr) {
+                if (x->layout() != at::kStrided) refuse(op, "params", i, "or what belongs to it is not strided");
+                if (x->device() != device) refuse(op, "params", i, "or what belongs to it is on another device");
+            }
+        t.param_type = element_type(p);
+        t.grad_type = element_type(g);
+        if (t.param_type < 0) refuse(op, "params", i, "must be float32, bfloat16 or float16");
+        if (t.grad_type < 0) refuse(op, "grads", i, "must be float32, bfloat16 or float16");
+        const bool contiguous = p.is_contiguous();
+        if (!contiguous && !p.is_non_overlapping_and_dense())
+            refuse(op, "params", i, "has gaps or overlaps in memory");
+        if (!same_layout(g, p, contiguous)) refuse(op, "grads", i, "is not laid out as its parameter");
+        if (mi.scalar_type() != state_type || !same_layout(mi, p, contiguous))
+            refuse(op, m.name, i, state_what);
+        if (vi.scalar_type() != state_type || !same_layout(vi, p, contiguous))
+            refuse(op, v.name, i, state_what);
+        t.numel = p.numel();
+        if (t.numel > (int64_t)1 << 34) refuse(op, "params", i, "has more than 2^34 elements");
+        t.param = p.data_ptr();
+        t.grad = g.data_ptr();
+        t.exp_avg = mi.data_ptr();
+        t.exp_avg_sq = vi.data_ptr();
+        t.exp_avg_scale = t.exp_avg_sq_scale = t.master = nullptr;
+        bool fresh = t.numel == 0 || (seen.add(t.param) && seen.add(t.exp_avg) && seen.add(t.exp_avg_sq));
+        if (w != nullptr) {
+            if (t.param_type == GI2D_F32) refuse(op, "masters", i, "belongs to a float32 parameter");
+            if (w->scalar_type() != at::kFloat || !same_layout(*w, p, contiguous))
+                refuse(op, "masters", i, "must be a float32 tensor laid out as its parameter");
+            t.master = t.numel ? w->data_ptr<float>() : nullptr;
+            fresh = fresh && (t.numel == 0 || seen.add(t.master));
+        }
+        if (!fresh) refuse(op, "params", i, "or its state appears twice");
+        if (bits == 8) {
+            const at::Tensor &a = *sm.at(i), &b = *sv.at(i);
+            const int64_t blocks = (t.numel + GI2D_ADAMW_BLOCK - 1) / GI2D_ADAMW_BLOCK;
+            for (const at::Tensor *x : {&a, &b})
+                if (x->scalar_type() != at::kFloat || x->numel() != blocks || !x->is_contiguous() ||
+                    x->device() != device)
+                    refuse(op, x == &a ? sm.name : sv.name, i,
+                           "must be a contiguous float32 tensor with one element for 256 of the "
+                           "parameter's, on its device");
+            if (t.numel) {
+                t.exp_avg_scale = a.data_ptr<float>();
+                t.exp_avg_sq_scale = b.data_ptr<float>();
+            }
+        }
+    }
+    need_gpu(op, *params.at(0));
+    gi2d_adamw_hyper h;
+    h.beta1 = beta1;
+    h.beta2 = beta2;
+    h.eps = eps;
+    h.weight_decay = weight_decay;
+    h.seed = seed;
+    h.state_bits = bits;
+    h.step = 1;
+    h.lr = 0.0;
+    h.step_dev = nullptr;
+    h.lr_dev = nullptr;
+    h.scalars_dev = nullptr;
+    const c10::DeviceGuard guard(device);
+    if (THPVariable_Check(step_.ptr()))
+        h.step_dev = device_scalar(op, "step", step_, at::kLong, device)->data_ptr<int64_t>();
+    else
+        h.step = step_.cast<int64_t>();
+    if (h.step < 1) throw py::value_error(std::string(op) + ": step counts from 1");
+    if (THPVariable_Check(lr_.ptr()))
+        h.lr_dev = device_scalar(op, "lr", lr_, at::kFloat, device)->data_ptr<float>();
+    else
+        h.lr = lr_.cast<double>();
+    at::Tensor scalars;  // (goes back to the allocator of this stream behind the launch)
+    if (h.step_dev != nullptr || h.lr_dev != nullptr) {
+        scalars = at::empty({GI2D_ADAMW_SCALARS_BYTES}, at::TensorOptions().dtype(at::kByte).device(device));
+        h.scalars_dev = scalars.data_ptr();
+    }
+    const float *clip = nullptr;
+    if (!clip_.is_none()) {
+        if (!THPVariable_Check(clip_.ptr()))
+            throw py::type_error(std::string(op) + ": clip must be a tensor (grad_norm's second result)");
+        clip = device_scalar(op, "clip", clip_, at::kFloat, device)->data_ptr<float>();
+    }
+    check(gi2d_adamw_step((int)n, ts.data(), &h, clip,
+                          c10::hip::getCurrentHIPStream(device.index()).stream()),
+          "gi2d_adamw_step", true);
+    for (int64_t i = 0; i < n; ++i) {
+        written(*params.at(i));
+        written(*m.at(i));
+        written(*v.at(i));
+        if (bits == 8) {
+            written(*sm.at(i));
+            written(*sv.at(i));
+        }
+        if (const at::Tensor *w = masters.at(i, true)) written(*w);
+    }
+}
+
+py::tuple grad_norm(const py::object &grads_, double max_norm)
+{
+    static const char *const op = "grad_norm";
+    const Tensors grads(grads_, "grads");
+    const int64_t n = grads.size();
+    if (n == 0) throw py::value_error("grad_norm: no gradients");
+    const at::Device device = grads.at(0)->device();
+    std::vector<const void *> ptr((size_t)n);
+    std::vector<int64_t> numel((size_t)n);
+    std::vector<int> type((size_t)n);
+    for (int64_t i = 0; i < n; ++i) {
+        const at::Tensor &g = *grads.at(i);
+        if (g.layout() != at::kStrided) refuse(op, "grads", i, "is not strided");
+        if (g.device() != device) refuse(op, "grads", i, "is on another device");
+        type[(size_t)i] = element_type(g);
+        if (type[(size_t)i] < 0) refuse(op, "grads", i, "must be float32, bfloat16 or float16");
+        if (!g.is_contiguous() && !g.is_non_overlapping_and_dense())
+            refuse(op, "grads", i, "has gaps or overlaps in memory");
+        numel[(size_t)i] = g.numel();
+        if (g.numel() > (int64_t)1 << 34) refuse(op, "grads", i, "has more than 2^34 elements");
+        ptr[(size_t)i] = g.numel() ? g.data_ptr() : nullptr;
+    }
+    need_gpu(op, *grads.at(0));
+    const c10::DeviceGuard guard(device);
+    const at::Tensor work = at::empty({gi2d_grad_norm_workspace((int)n)},
+                                      at::TensorOptions().dtype(at::kByte).device(device));
+    const at::Tensor out = at::empty({2}, at::TensorOptions().dtype(at::kFloat).device(device));
+    check(gi2d_grad_norm((int)n, ptr.data(), numel.data(), type.data(), max_norm, work.data_ptr(),
+                         out.data_ptr<float>(), c10::hip::getCurrentHIPStream(device.index()).stream()),
+          "gi2d_grad_norm", true);
+    return py::make_tuple(out.select(0, 0), out.select(0, 1));
+}
+
+}  // namespace adamw

@@ -6,8 +6,10 @@
 // libgi2d.so.  The Python binding (ops.py) has the same behaviour and is what this replaces on
 // the hot path: argument checks, per-stream workspaces, the tile lists shared by the raster
 // passes of one model forward, the handling of a late overflow report.
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
 
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
 #include <climits>
@@ -501,6 +503,8 @@ at::Tensor py_rasterize_sum(const at::Tensor &xys, const at::Tensor &radii, cons
                           (int)W);
 }
 
+#include "torch_adamw.h"
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
@@ -535,4 +539,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     m.def("project_gaussians_2d", &py_project_gaussians_2d);
     m.def("project_gaussians_2d_scale_rot", &py_project_gaussians_2d_scale_rot);
     m.def("rasterize_gaussians_sum", &py_rasterize_sum);
+    m.def("adamw_step", &adamw::step);
+    m.def("grad_norm", &adamw::grad_norm);
 }

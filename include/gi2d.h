@@ -304,6 +304,61 @@ int gi2d_adan_step(int num_tensors, float *const *params, float *const *grads,
                    float *const *neg_pre_grad, const int64_t *numel, const gi2d_adan_hyper *hyper,
                    const float *clip_dev, void *stream);
 
+/* AdamW step over a list of tensors (decoupled weight decay; t = step count, 1 for the first):
+ *   m = b1 m + (1-b1) g,  v = b2 v + (1-b2) g^2,
+ *   p = p (1 - lr wd) - lr/(1-b1^t) * m / (sqrt(v)/sqrt(1-b2^t) + eps).
+ * Parameters and gradients are fp32, bf16 or fp16, each tensor its own; arithmetic is fp32.  A half
+ * parameter may have an fp32 master, which is then what is read and updated, the parameter its
+ * rounding.  The gradients are not written.  One launch per 64 tensors (48 with 8-bit states) of
+ * the same types; nothing is allocated and nothing is read on the host, so a call may be captured.
+ * No element may appear twice among what a call writes.
+ * state_bits 32: exp_avg and exp_avg_sq are fp32.
+ * state_bits 8: for GI2D_ADAMW_BLOCK consecutive elements one power-of-two scale and one e4m3 code
+ * each: m = code * scale, sqrt(v) = code * scale.  exp_avg / exp_avg_sq hold the codes (numel
+ * bytes; all-zero codes are a fresh state whatever the scales), the scales are fp32, one for each
+ * block.  The codes are rounded at random with the mean kept, by a hash of (seed, step, block,
+ * element): the same call gives the same bits.  Infinities and NaN become the NaN code. */
+#define GI2D_F32 0
+#define GI2D_BF16 1
+#define GI2D_F16 2
+#define GI2D_ADAMW_BLOCK 256
+#define GI2D_ADAMW_SCALARS_BYTES 64
+typedef struct gi2d_adamw_tensor {
+    void *param;
+    const void *grad;
+    void *exp_avg;
+    void *exp_avg_sq;
+    float *exp_avg_scale;    /* state_bits 8 only */
+    float *exp_avg_sq_scale; /* state_bits 8 only */
+    float *master;           /* NULL = none */
+    int64_t numel;           /* at most 2^34 */
+    int param_type, grad_type;
+} gi2d_adamw_tensor;
+typedef struct gi2d_adamw_hyper {
+    double lr, beta1, beta2, eps, weight_decay;
+    int64_t step;
+    uint32_t seed; /* state_bits 8 only */
+    int state_bits;
+    /* for captured steps: the step count and the learning rate in device memory (either may be
+     * NULL), read when the step runs; scalars_dev: GI2D_ADAMW_SCALARS_BYTES of device memory that
+     * belong to this call until it has run */
+    const int64_t *step_dev;
+    const float *lr_dev;
+    void *scalars_dev;
+} gi2d_adamw_hyper;
+/* `tensors` is a host array.  clip_dev: optional device scalar the gradients are multiplied by as
+ * they are read (out[1] of gi2d_grad_norm), NULL = 1. */
+int gi2d_adamw_step(int num_tensors, const gi2d_adamw_tensor *tensors,
+                    const gi2d_adamw_hyper *hyper, const float *clip_dev, void *stream);
+
+/* 2-norm of all gradients together: out[0] = sqrt(sum g^2), summed in double and in a fixed order,
+ * out[1] = min(1, max_norm / (out[0] + 1e-6)).  Host arrays of device pointers, element counts and
+ * element types; `workspace`: gi2d_grad_norm_workspace(num_tensors) bytes of device memory that
+ * belong to this call until it has run; out: two floats in device memory. */
+int64_t gi2d_grad_norm_workspace(int num_tensors);
+int gi2d_grad_norm(int num_tensors, const void *const *grads, const int64_t *numel,
+                   const int *types, double max_norm, void *workspace, float *out, void *stream);
+
 /* Fused fitting iteration on the model's RAW parameters -- the caller's loop of
  * gaussianimage_cholesky.py:101-124 / gaussianimage_rs.py:82-95 (forward, L2
  * loss, backward, Adan step) in FOUR launches (three with the chained step

@@ -1,0 +1,883 @@
+"""AdamW over lists of tensors (32-bit and 8-bit states) and the gradient norm.
+
+CPU: the float64 restatement (oracle/adamw_oracle.py) against torch.optim.AdamW in float64, the
+properties of the 8-bit rounding, and every refusal.  GPU: the kernels against the restatement,
+with the bounds that it counts rounding by rounding."""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import adamw_oracle as O
+
+DEV = "cuda:0"
+BETAS, EPS, DECAY, LR = (0.9, 0.999), 1e-8, 1e-2, 1e-3
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+E4M3 = torch.float8_e4m3fn
+
+
+# ------------------------------------------------------------------ CPU: the restatement
+
+def test_restatement_follows_torch_in_double():
+    g = torch.Generator().manual_seed(1)
+    p = torch.nn.Parameter(torch.randn(50, generator=g, dtype=torch.float64))
+    opt = torch.optim.AdamW([p], lr=LR, betas=BETAS, eps=EPS, weight_decay=DECAY)
+    q, m, v = p.detach().numpy().copy(), np.zeros(50), np.zeros(50)
+    for t in range(1, 9):
+        p.grad = torch.randn(50, generator=g, dtype=torch.float64)
+        opt.step()
+        q, m, v, *_ = O.step(q, p.grad.numpy(), m, v, t, LR, BETAS, EPS, DECAY)
+        assert np.allclose(q, p.detach().numpy(), rtol=1e-12, atol=1e-14)
+
+
+def test_restated_codes_are_torch_e4m3():
+    codes = torch.arange(128, dtype=torch.uint8)
+    assert np.array_equal(codes.view(E4M3).double().numpy(), O.e4m3_values(), equal_nan=True)
+
+
+def test_rounding_keeps_the_mean_and_what_is_exact():
+    x = np.abs(np.random.RandomState(3).randn(BLK := 256)) * 0.01
+    seeds = 4000
+    total = np.zeros(BLK)
+    for s in range(seeds):
+        r = O.words(s, 5, 0, BLK)
+        c, k, _ = O.encode(x, r >> np.uint64(16), False)
+        total += O.decode(c, k, BLK)
+    values = O.e4m3_values()[:127]
+    y = x / k[0]
+    lo = np.searchsorted(values, y, side="right") - 1
+    gap = (values[np.minimum(lo + 1, 126)] - values[lo]) * k[0]
+    # standard deviation of one rounding is at most half a gap
+    assert np.all(np.abs(total / seeds - x) <= 6 * 0.5 * gap / math.sqrt(seeds) + gap * 2.0 ** -16)
+    # a value on the grid keeps its code whatever the random number
+    for r in (0, 1, 65535):
+        c2, k2, _ = O.encode(O.decode(c, k, BLK), np.full(BLK, r, np.uint64), False)
+        assert np.array_equal(c2, c) and np.array_equal(k2, k)
+
+
+# ------------------------------------------------------------------ CPU: refusals
+
+def _cpu(n=300, dtype=F32):
+    p = torch.zeros(n, dtype=dtype)
+    return [p], [torch.zeros(n, dtype=dtype)], [torch.zeros(n)], [torch.zeros(n)]
+
+
+@pytest.fixture(params=["compiled", "ctypes"])
+def binding(request):
+    from gaussianimage_amd import ops
+    previous = ops.use_compiled(request.param == "compiled")
+    yield request.param
+    ops.use_compiled(previous)
+
+
+def test_refused_hyperparameters():
+    from gaussianimage_amd.adamw import AdamW, adamw_step, adamw_step_8bit, grad_norm
+    p = [torch.nn.Parameter(torch.zeros(3))]
+    for bad in (dict(lr=-1.0), dict(eps=-1.0), dict(betas=(1.0, 0.9)), dict(betas=(0.9, -0.1)),
+                dict(betas=(0.9,)), dict(weight_decay=-0.1), dict(max_grad_norm=-1.0),
+                dict(state_bits=16), dict(seed=-1), dict(seed=2 ** 32), dict(lr=float("nan"))):
+        with pytest.raises(ValueError):
+            AdamW(p, **bad)
+    for bad in (dict(lr=-1.0), dict(eps=-1.0), dict(betas=(0.9, 1.0)), dict(weight_decay=-1.0)):
+        with pytest.raises(ValueError):
+            adamw_step(*_cpu(), step=1, **bad)
+        with pytest.raises(ValueError):
+            adamw_step_8bit([], [], [], [], [], [], step=1, **bad)
+    with pytest.raises(ValueError):
+        grad_norm([torch.zeros(3)], max_norm=-1.0)
+    with pytest.raises(ValueError):
+        grad_norm([torch.zeros(3)], max_norm=float("nan"))
+
+
+def test_refused_tensors(binding):
+    from gaussianimage_amd.adamw import adamw_step, adamw_step_8bit, grad_norm, zero_state_8bit
+    p, g, m, v = _cpu()
+    step = lambda *a, **k: adamw_step(*a, **{"step": 1, **k})  # noqa: E731
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        step(p, g, m, v)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        grad_norm(g)
+    for wrong in range(1, 4):                        # another number of tensors
+        lists = [p, g, m, v]
+        lists[wrong] = lists[wrong] * 2
+        with pytest.raises(ValueError, match="entries"):
+            step(*lists)
+    with pytest.raises(ValueError, match="entries"):
+        step(p, g, m, v, masters=[])
+    with pytest.raises(TypeError, match="not a tensor"):
+        step(p, [None], m, v)
+    with pytest.raises(ValueError, match="float32, bfloat16 or float16"):
+        step([torch.zeros(300, dtype=torch.float64)], g, m, v)
+    with pytest.raises(ValueError, match="float32, bfloat16 or float16"):
+        step(p, [torch.zeros(300, dtype=torch.int32)], m, v)
+    with pytest.raises(ValueError, match="laid out"):
+        step(p, [torch.zeros(299)], m, v)
+    with pytest.raises(ValueError, match="laid out"):
+        step(p, g, [torch.zeros(300, dtype=BF16)], v)
+    with pytest.raises(ValueError, match="laid out"):
+        step(p, g, m, [torch.zeros(300, 1)])
+    with pytest.raises(ValueError, match="strided"):
+        step(p, [torch.zeros(300).to_sparse()], m, v)
+    with pytest.raises(ValueError, match="gaps or overlaps"):
+        step([torch.zeros(600)[::2]], g, m, v)
+    with pytest.raises(ValueError, match="gaps or overlaps"):
+        step([torch.zeros(1).expand(300)], g, m, v)
+    square, turned = torch.zeros(4, 6), torch.zeros(6, 4).t()
+    with pytest.raises(ValueError, match="laid out"):
+        step([turned], [square], [square], [square.clone()])
+    with pytest.raises(ValueError, match="another device"):
+        step(p, [torch.zeros(300, device="meta")], m, v)
+    with pytest.raises(ValueError, match="twice"):
+        step(p * 2, g * 2, m + [torch.zeros(300)], v + [torch.zeros(300)])
+    with pytest.raises(ValueError, match="twice"):
+        step(p, g, m, m)
+    with pytest.raises(ValueError, match="belongs to a float32"):
+        step(p, g, m, v, masters=[torch.zeros(300)])
+    half = torch.zeros(300, dtype=BF16)
+    with pytest.raises(ValueError, match="masters"):
+        step([half], [half.clone()], m, v, masters=[torch.zeros(300, dtype=BF16)])
+    a, sa, b, sb = zero_state_8bit(p[0])
+    assert a.dtype == E4M3 and sa.shape == (2,)
+    eight = lambda *x, **k: adamw_step_8bit(p, g, *[[t] for t in x], **{"step": 1, **k})  # noqa: E731
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        eight(a, sa, b, sb)
+    with pytest.raises(ValueError, match="float8_e4m3fn|Float8_e4m3fn"):
+        eight(m[0], sa, b, sb)
+    with pytest.raises(ValueError, match="exp_avg_scales"):
+        eight(a, sa[:1], b, sb)
+    with pytest.raises(ValueError, match="exp_avg_rms_scales"):
+        eight(a, sa, b, sb.double())
+    with pytest.raises(ValueError, match="twice"):
+        eight(a, sa, a, sb)
+    with pytest.raises(ValueError, match="no gradients"):
+        grad_norm([])
+    with pytest.raises(ValueError, match="gaps"):
+        grad_norm([torch.zeros(1).expand(5)])
+    with pytest.raises(ValueError, match="float32, bfloat16 or float16"):
+        grad_norm([torch.zeros(3, dtype=torch.float64)])
+    step([], [], [], [])                             # nothing to do is no error
+
+
+def test_optimizer_refuses_cpu_parameters():
+    from gaussianimage_amd.adamw import AdamW
+    p = [torch.nn.Parameter(torch.zeros(3))]
+    for bits in (32, 8):
+        opt = AdamW(p, state_bits=bits)
+        opt.step()                                   # no gradients: nothing happens
+        p[0].grad = torch.ones(3)
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            opt.step()
+        p[0].grad = None
+
+
+def test_c_entries_refuse_without_a_device():
+    from gaussianimage_amd import _lib
+    lib, bad = _lib.lib, _lib.GI2D_E_INVALID
+
+    def hyper(**kw):
+        return ctypes.byref(_lib.AdamWHyper(**{**dict(lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8,
+                                                      step=1, state_bits=32), **kw}))
+
+    def table(**kw):
+        t = (_lib.AdamWTensor * 1)()
+        for k, x in {**dict(param=64, grad=64, exp_avg=64, exp_avg_sq=64, numel=4), **kw}.items():
+            setattr(t[0], k, x)
+        return t
+
+    assert lib.gi2d_adamw_step(0, None, hyper(), None, None) == _lib.GI2D_OK
+    assert lib.gi2d_adamw_step(1, table(numel=0), hyper(), None, None) == _lib.GI2D_OK
+    assert lib.gi2d_adamw_step(-1, None, hyper(), None, None) == bad
+    assert lib.gi2d_adamw_step(1, None, hyper(), None, None) == bad
+    assert lib.gi2d_adamw_step(0, None, None, None, None) == bad
+    for kw in (dict(step=0), dict(state_bits=4), dict(beta1=1.0), dict(beta2=-0.1),
+               dict(beta1=float("nan")), dict(step_dev=64), dict(lr_dev=64)):
+        assert lib.gi2d_adamw_step(1, table(), hyper(**kw), None, None) == bad, kw
+    for kw in (dict(param=None), dict(grad=None), dict(exp_avg=None), dict(exp_avg_sq=None),
+               dict(numel=-1), dict(numel=2 ** 34 + 1), dict(param_type=3), dict(grad_type=-1),
+               dict(master=64)):
+        assert lib.gi2d_adamw_step(1, table(**kw), hyper(), None, None) == bad, kw
+    assert lib.gi2d_adamw_step(1, table(), hyper(state_bits=8), None, None) == bad
+    assert lib.gi2d_grad_norm_workspace(-1) == bad
+    assert lib.gi2d_grad_norm_workspace(0) > 0
+    assert lib.gi2d_grad_norm_workspace(129) == 2 * lib.gi2d_grad_norm_workspace(128)
+    one = (ctypes.c_void_p * 1)(64)
+    size, kind = (ctypes.c_int64 * 1)(4), (ctypes.c_int * 1)(0)
+    for a in ((-1, one, size, kind, 1.0, 64, 64), (1, None, size, kind, 1.0, 64, 64),
+              (1, one, None, kind, 1.0, 64, 64), (1, one, size, None, 1.0, 64, 64),
+              (1, one, size, kind, -1.0, 64, 64), (1, one, size, kind, float("nan"), 64, 64),
+              (1, one, size, kind, 1.0, None, 64), (1, one, size, kind, 1.0, 64, None),
+              (1, (ctypes.c_void_p * 1)(None), size, kind, 1.0, 64, 64),
+              (1, one, (ctypes.c_int64 * 1)(-1), kind, 1.0, 64, 64),
+              (1, one, size, (ctypes.c_int * 1)(3), 1.0, 64, 64)):
+        assert lib.gi2d_grad_norm(*a, None) == bad, a
+
+
+# ------------------------------------------------------------------ GPU: helpers
+
+class Case:
+    """Tensors of the given element counts, with guard elements around each (``off`` elements
+    before it: alignments an allocator would not give), and their float64 images."""
+
+    def __init__(self, sizes, pt, gt, bits, master=False, off=0, seed=0, gscale=1e-2):
+        rng = np.random.RandomState(seed)
+        self.sizes, self.bits = sizes, bits
+        self.guards = []
+        self.np = []
+        self.cols = {k: [] for k in ("p", "g", "m", "v", "sm", "sv", "w")}
+        for n in sizes:
+            scale = 2.0 ** rng.uniform(-6, 2, size=-(-n // 256) or 1).repeat(256)[:n] * gscale
+            w = self.put(rng.randn(n) * 0.05, F32 if master else pt, off)
+            p = self.put(w.double().cpu().numpy(), pt, off) if master else w
+            g = self.put(rng.randn(n) * scale, gt, off)
+            m, r = rng.randn(n) * scale * 0.3, np.abs(rng.randn(n)) * scale + 0.05 * scale
+            if bits == 32:
+                m, v, sm, sv = self.put(m, F32, off), self.put(r * r, F32, off), None, None
+                m64, v64 = m.double().cpu().numpy(), v.double().cpu().numpy()
+            else:
+                half = np.full(n, 32767, np.uint64)
+                cm, km, _ = O.encode(m, half, False)
+                cr, kr, _ = O.encode(r, half, True)
+                m64, v64 = O.decode(cm, km, n), O.decode(cr, kr, n) ** 2
+                m, v = self.put(cm, torch.uint8, off).view(E4M3), self.put(cr, torch.uint8, off).view(E4M3)
+                sm, sv = self.put(km, F32, 0), self.put(kr, F32, 0)
+            for k, x in zip(self.cols, (p, g, m, v, sm, sv, w if master else None)):
+                self.cols[k].append(x)
+            self.np.append((w.double().cpu().numpy(), g.double().cpu().numpy(), m64, v64))
+
+    def put(self, x, dtype, off):
+        x = torch.as_tensor(np.asarray(x))
+        n = x.numel()
+        buf = torch.full((n + off + 8,), 77, dtype=dtype, device=DEV)
+        view = buf[off:off + n]
+        view.copy_(x)
+        self.guards.append((buf, off, n))
+        return view
+
+    def run(self, t=7, clip=None, seed=11, lr=LR, betas=BETAS, eps=EPS, wd=DECAY):
+        from gaussianimage_amd.adamw import adamw_step, adamw_step_8bit
+        c = self.cols
+        masters = c["w"] if any(x is not None for x in c["w"]) else None
+        kw = dict(step=t, lr=lr, betas=betas, eps=eps, weight_decay=wd, masters=masters, clip=clip)
+        if self.bits == 32:
+            adamw_step(c["p"], c["g"], c["m"], c["v"], **kw)
+        else:
+            adamw_step_8bit(c["p"], c["g"], c["m"], c["sm"], c["v"], c["sv"], seed=seed, **kw)
+
+    def check(self, t=7, clip=1.0, seed=11, lr=LR, betas=BETAS, eps=EPS, wd=DECAY):
+        block, wrong, total = 0, 0, 0
+        for i, n in enumerate(self.sizes):
+            w, g, m, v = self.np[i]
+            p2, m2, v2, tp, tm, tv = O.step(w, g, m, v, t, lr, betas, eps, wd, clip)
+            p, master = self.cols["p"][i], self.cols["w"][i]
+            if master is not None:
+                _near(master, p2, tp, f"master {i}")
+                assert torch.equal(p, master.to(p.dtype)), f"parameter {i} is not its master's rounding"
+            elif p.dtype == F32:
+                _near(p, p2, tp, f"parameter {i}")
+            else:
+                info = torch.finfo(p.dtype)
+                half = np.maximum(np.abs(p2) * info.eps / 2, info.tiny * info.eps / 2)
+                _near(p, p2, tp * (1 + info.eps) + half, f"parameter {i}")
+            if self.bits == 32:
+                _near(self.cols["m"][i], m2, tm, f"mean {i}")
+                _near(self.cols["v"][i], v2, tv, f"square {i}")
+            else:
+                r = O.words(seed, t, block, n)
+                root = np.sqrt(v2)
+                tol_r = tv / (2 * np.maximum(root, 1e-30)) + 2 * O.u * root
+                for col, sc, x, tol, bits, nz in (("m", "sm", m2, tm, r >> np.uint64(16), False),
+                                                  ("v", "sv", root, tol_r, r & np.uint64(65535), True)):
+                    want, scales, margin = O.encode(x, bits, nz)
+                    got = self.cols[col][i].view(torch.uint8).cpu().numpy()
+                    assert np.array_equal(self.cols[sc][i].cpu().numpy(), scales), f"scales {col} {i}"
+                    # Another code only where the value before rounding may be on the other side of
+                    # the random number; the position itself is kept to 2^-21 of a step.
+                    values = O.e4m3_values()[:127]
+                    at = np.minimum(want & 127, 125)
+                    step = (values[at + 1] - values[at]) * np.repeat(scales, 256)[:n]
+                    tol = tol + 2.0 ** -20 * step
+                    off = (got != want) & ((got | want) & 127 != 0)  # (zeros of both signs are equal)
+                    assert np.all(margin[off] <= tol[off]), f"codes {col} {i}"
+                    diff = np.abs((got[off] & 127).astype(int) - (want[off] & 127))
+                    assert np.all(diff <= 1), f"codes {col} {i}"
+                    wrong += int(off.sum())
+                    # the random numbers are even, so of all values 2 tol / step are that near (a
+                    # step may be half as long on the other side)
+                    total += float(np.minimum(1.0, 4 * tol / step).sum()) if n else 0.0
+                block += -(-n // 256)
+        assert wrong <= 8 + 2 * total
+        self.check_guards()
+
+    def check_guards(self):
+        for buf, off, n in self.guards:
+            around = torch.cat([buf[:off], buf[off + n:]]).float()
+            assert torch.all(around == 77), "wrote outside a tensor"
+
+
+def _near(got, want, tol, what):
+    got = got.detach().double().cpu().numpy()
+    assert got.shape == want.shape
+    assert np.array_equal(np.isnan(got), np.isnan(want)), what
+    fine = np.isfinite(want)
+    assert np.array_equal(got[~fine & ~np.isnan(want)], want[~fine & ~np.isnan(want)]), what
+    worst = np.max((np.abs(got - want) - tol)[fine], initial=-1.0)
+    assert worst <= 0, f"{what}: off by {worst} more than the bound"
+
+
+TYPES = [(F32, F32, False), (F32, BF16, False), (F32, F16, False), (BF16, BF16, False),
+         (BF16, F32, False), (F16, F16, False), (F16, F32, True), (BF16, BF16, True),
+         (BF16, F32, True), (F16, F16, True), (F16, BF16, False), (BF16, F16, True)]
+IDS = [f"{str(p)[6:]}-{str(g)[6:]}{'-master' if m else ''}" for p, g, m in TYPES]
+SIZES = [1, 2, 3, 255, 256, 257, 0, 2047, 2048, 2049, 4096, 5003]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("off", [0, 1, 4])
+@pytest.mark.parametrize("pt,gt,master", TYPES, ids=IDS)
+def test_step(bits, pt, gt, master, off, binding):
+    c = Case(SIZES, pt, gt, bits, master, off, seed=off + 1)
+    c.run()
+    c.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("t,betas,eps,wd,lr", [
+    (1, BETAS, EPS, DECAY, LR), (2, (0.0, 0.0), 1e-6, 0.0, 0.1), (100000, (0.95, 0.9999), 1e-12, 0.3, 1e-2),
+    (3, BETAS, 0.0, DECAY, 0.0)])
+def test_hyperparameters(bits, t, betas, eps, wd, lr):
+    c = Case([1000, 300], F32, F32, bits, seed=t)
+    c.run(t=t, betas=betas, eps=eps, wd=wd, lr=lr)
+    c.check(t=t, betas=betas, eps=eps, wd=wd, lr=lr)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_clip_coefficient(bits):
+    c = Case([700, 2100], F32, BF16, bits, seed=5)
+    coef = torch.tensor(0.3, device=DEV)
+    before = [g.clone() for g in c.cols["g"]]
+    c.run(clip=coef)
+    c.check(clip=float(coef))
+    assert all(torch.equal(a, b) for a, b in zip(before, c.cols["g"]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_many_tensors_of_mixed_types(bits):
+    """More tensors than a launch takes, of all types in turn: the words of the 8-bit rounding
+    count blocks over the whole list."""
+    from gaussianimage_amd.adamw import adamw_step, adamw_step_8bit
+    rng = np.random.RandomState(2)
+    parts = [Case([int(rng.randint(0, 1500))], *TYPES[i % len(TYPES)][:2], bits,
+                  TYPES[i % len(TYPES)][2], seed=100 + i) for i in range(150)]
+    col = lambda k: [c.cols[k][0] for c in parts]  # noqa: E731
+    kw = dict(step=7, lr=LR, betas=BETAS, eps=EPS, weight_decay=DECAY, masters=col("w"))
+    if bits == 32:
+        adamw_step(col("p"), col("g"), col("m"), col("v"), **kw)
+    else:
+        adamw_step_8bit(col("p"), col("g"), col("m"), col("sm"), col("v"), col("sv"), seed=11, **kw)
+    whole = parts[0]
+    whole.sizes = [c.sizes[0] for c in parts]
+    whole.np = [c.np[0] for c in parts]
+    whole.cols = {k: col(k) for k in whole.cols}
+    whole.guards = [g for c in parts for g in c.guards]
+    whole.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_dense_strides(bits):
+    """A parameter in another order than its sizes': everything in the same order."""
+    from gaussianimage_amd.adamw import adamw_step, adamw_step_8bit
+    flat = Case([60 * 40], F32, F32, bits, seed=9)
+    c = {k: [None if x[0] is None or k in ("sm", "sv") else x[0].view(40, 60).t()] for k, x in flat.cols.items()}
+    assert not c["p"][0].is_contiguous()
+    kw = dict(step=7, lr=LR, betas=BETAS, eps=EPS, weight_decay=DECAY)
+    if bits == 32:
+        adamw_step(c["p"], c["g"], c["m"], c["v"], **kw)
+    else:
+        adamw_step_8bit(c["p"], c["g"], c["m"], flat.cols["sm"], c["v"], flat.cols["sv"], seed=11, **kw)
+    flat.check()
+
+
+@pytest.mark.gpu
+def test_special_values_32():
+    """Zeros, infinities, NaN and squares beyond float32 follow the formula."""
+    from gaussianimage_amd.adamw import adamw_step
+    g = torch.tensor([0.0, float("inf"), float("nan"), -float("inf"), 1e30, 1e-30, 0.0], device=DEV)
+    p, m, v = torch.ones(7, device=DEV), torch.zeros(7, device=DEV), torch.zeros(7, device=DEV)
+    m[6], v[6] = 1e-3, 0.0                           # a zero square under a mean: divided by eps
+    adamw_step([p], [g], [m], [v], step=1, lr=1e-9, betas=BETAS, eps=EPS, weight_decay=0.0)
+    p, m, v = p.cpu(), m.cpu(), v.cpu()
+    assert p[0] == 1 and m[0] == 0 and v[0] == 0
+    assert all(torch.isnan(p[i]) for i in (1, 2, 3)) and torch.isnan(m[2]) and torch.isinf(m[3])
+    assert p[4] == 1 and torch.isinf(v[4])           # a mean over an infinite root
+    assert torch.isfinite(p[5]) and v[5] == 0
+    assert abs(float(p[6]) - (1 - 1e-9 * (1e-3 * 0.9 / 0.1) / 1e-8)) <= 1e-6
+
+
+@pytest.mark.gpu
+def test_special_values_8():
+    """What is not finite becomes the NaN code and leaves the rest of its block alone."""
+    bad = {3: float("inf"), 17: float("nan"), 40: -float("inf")}
+    a, b = (Case([700], F32, F32, 8, seed=4) for _ in range(2))
+    for i, x in bad.items():
+        a.cols["g"][0][i] = x
+    a.run()
+    b.run()
+    keep = torch.ones(700, dtype=torch.bool, device=DEV)
+    keep[list(bad)] = False
+    for k in ("m", "v"):
+        x, y = (c.cols[k][0].view(torch.uint8) for c in (a, b))
+        assert torch.all((x[~keep] & 127) == 127)
+        assert torch.equal(x[256:], y[256:])
+        # (the block's scales need no change: the three were not its largest)
+    for k in ("sm", "sv"):
+        x, y = a.cols[k][0], b.cols[k][0]
+        assert torch.equal(x[1:], y[1:]) and 0.5 <= float(x[0] / y[0]) <= 1.0
+    assert torch.equal(a.cols["p"][0][keep], b.cols["p"][0][keep])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [1e-36, 1e-18, 1e18, 1e37])
+def test_magnitudes_8(size):
+    """Scales at both ends of their range; blocks of zeros."""
+    from gaussianimage_amd.adamw import adamw_step_8bit, zero_state_8bit
+    n = 600
+    x = np.random.RandomState(1).randn(n)
+    g = torch.tensor(x * size, dtype=F32, device=DEV)
+    g[256:512] = 0
+    p = torch.ones(n, device=DEV)
+    m, sm, r, sr = zero_state_8bit(p)
+    adamw_step_8bit([p], [g], [m], [sm], [r], [sr], step=1, lr=LR, betas=(0.5, 0.5), eps=0.0 if size > 1 else EPS,
+                    weight_decay=0.0, seed=3)
+    mean = g.double() * 0.5
+    got = m.float().double() * sm.double().repeat_interleave(256)[:n]
+    # one step of the code: 1/8 of the value, or the smallest one at the smallest scale
+    assert torch.all((got - mean).abs() <= mean.abs() / 8 + sm.double().repeat_interleave(256)[:n] * 2.0 ** -9)
+    assert torch.all(m.view(torch.uint8)[256:512] == 0) and torch.all(r.view(torch.uint8)[256:512] == 0)
+    assert torch.all(sm > 0) and torch.all(torch.isfinite(sm)) and torch.all(sr > 0)
+    if 1e-19 < size < 1e19:
+        root = (g.double() ** 2 * 0.5).sqrt()
+        got = r.float().double() * sr.double().repeat_interleave(256)[:n]
+        assert torch.all((got - root).abs() <= root / 8 + sr.double().repeat_interleave(256)[:n] * 2.0 ** -9)
+    elif size > 1:                                   # squares beyond float32: the NaN code
+        assert torch.all((r.view(torch.uint8)[:256] == 127) == torch.isinf((g * g * 0.5)[:256]))
+
+
+@pytest.mark.gpu
+def test_a_root_that_is_not_zero_stays_so():
+    from gaussianimage_amd.adamw import adamw_step_8bit, zero_state_8bit
+    n = 256
+    g = torch.full((n,), 1e-7, device=DEV)
+    g[0] = 1.0
+    p = torch.zeros(n, device=DEV)
+    m, sm, r, sr = zero_state_8bit(p)
+    for t in range(1, 6):
+        adamw_step_8bit([p], [g], [m], [sm], [r], [sr], step=t, lr=LR, betas=BETAS, eps=EPS, weight_decay=0.0)
+        assert torch.all(r.view(torch.uint8) > 0)
+    g.zero_()
+    before = p.clone()
+    adamw_step_8bit([p], [g], [m], [sm], [r], [sr], step=6, lr=LR, betas=BETAS, eps=EPS, weight_decay=0.0)
+    # |m| <= 3.2 sqrt(v) at these betas, whatever was rounded up: no step of lr * m / eps
+    assert torch.all((p - before).abs() <= 20 * LR)
+
+
+@pytest.mark.gpu
+def test_rounding_on_the_gpu_keeps_the_mean():
+    from gaussianimage_amd.adamw import adamw_step_8bit, zero_state_8bit
+    n, runs = 512, 600
+    g = torch.tensor(np.abs(np.random.RandomState(8).randn(n)) * 1e-3 + 1e-4, dtype=F32, device=DEV)
+    total, root = torch.zeros(n, dtype=torch.float64, device=DEV), torch.zeros(n, dtype=torch.float64, device=DEV)
+    for s in range(runs):
+        p = torch.zeros(n, device=DEV)
+        m, sm, r, sr = zero_state_8bit(p)
+        adamw_step_8bit([p], [g], [m], [sm], [r], [sr], step=1, seed=s)
+        total += m.float().double() * sm.double().repeat_interleave(256)
+        root += r.float().double() * sr.double().repeat_interleave(256)
+    for got, want, k in ((total / runs, g.double() * (1 - 0.9), sm), (root / runs, g.double() * math.sqrt(1 - 0.999), sr)):
+        gap = torch.maximum(want / 8, k.double().repeat_interleave(256) * 2.0 ** -9)
+        assert torch.all((got - want).abs() <= 6 * 0.5 * gap / math.sqrt(runs) + gap * 2.0 ** -12)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_more_than_2_31_elements(bits):
+    """Offsets beyond 32 bits: the ends of one long bfloat16 tensor against the same elements as
+    short tensors (32 bits: the same bits; 8 bits: the blocks' numbers differ, so parameters and
+    scales)."""
+    n = 2 ** 31 + 3 * 2048 + 77
+    free, _ = torch.cuda.mem_get_info()
+    if free < n * (14 if bits == 32 else 8):
+        pytest.skip("not enough device memory")
+    from gaussianimage_amd.adamw import adamw_step, adamw_step_8bit, grad_norm, zero_state_8bit
+    p, g = (torch.zeros(n, dtype=BF16, device=DEV) for _ in range(2))
+    tail = 5 * 2048 + 77
+    x = torch.randn(tail, device=DEV)
+    p[-tail:], g[-tail:] = x, torch.randn(tail, device=DEV)
+    q, h = p[-tail:].clone(), g[-tail:].clone()
+    norm, _ = grad_norm([g], 1.0)
+    want = h.double().square().sum().sqrt()
+    assert abs(float(norm) - float(want)) <= 4 * O.u * float(want)
+    if bits == 32:
+        s = [torch.zeros(n, device=DEV) for _ in range(2)]
+        z = [torch.zeros(tail, device=DEV) for _ in range(2)]
+        adamw_step([p], [g], [s[0]], [s[1]], step=1)
+        adamw_step([q], [h], [z[0]], [z[1]], step=1)
+        for a, b in ((p, q), (s[0], z[0]), (s[1], z[1])):
+            assert torch.equal(a[-tail:], b)
+            assert not a[:-tail].any()
+    else:
+        s, z = zero_state_8bit(p), zero_state_8bit(q)
+        adamw_step_8bit([p], [g], *[[t] for t in s], step=1)
+        adamw_step_8bit([q], [h], *[[t] for t in z], step=1)
+        assert torch.equal(p[-tail:], q) and not p[:-tail].any()
+        blocks = -(-tail // 256)
+        assert torch.equal(s[1][-blocks:], z[1]) and torch.equal(s[3][-blocks:], z[3])
+        for a, b in ((s[0], z[0]), (s[2], z[2])):
+            a, b = a.view(torch.uint8), b.view(torch.uint8)
+            assert not a[:-tail].any()
+            assert int((a[-tail:].short() - b.short()).abs().max()) <= 1
+
+
+# ------------------------------------------------------------------ GPU: the norm
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("off", [0, 1])
+@pytest.mark.parametrize("types", [[F32], [BF16], [F16], [F32, BF16, F16]], ids=["f32", "bf16", "f16", "mixed"])
+def test_grad_norm(types, off, binding):
+    from gaussianimage_amd.adamw import grad_norm
+    rng = np.random.RandomState(3)
+    sizes = [1, 0, 7, 4095, 4096, 4097, 8191, 8192, 8193, 100003] + [int(rng.randint(1, 300)) for _ in range(200)]
+    grads = []
+    for i, n in enumerate(sizes):
+        buf = torch.full((n + off,), float("nan"), dtype=types[i % len(types)], device=DEV)
+        buf[off:] = torch.as_tensor(rng.randn(n))
+        grads.append(buf[off:])
+    for limit in (0.0, 1.0, 1e9):
+        norm, coef = grad_norm(grads, limit)
+        want, c = O.grad_norm([g.double().cpu().numpy() for g in grads], limit)
+        assert norm.shape == coef.shape == () and norm.dtype == F32 and norm.device == coef.device == grads[0].device
+        # the sum in double, then one rounding to float, its root and the power of two: 2 roundings;
+        # the coefficient 3 more
+        assert abs(float(norm) - want) <= 2 * O.u * want
+        assert abs(float(coef) - c) <= 5 * O.u * c
+    again, none = grad_norm(grads)
+    assert torch.equal(again, norm) and none is None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [1e-44, 1e-30, 1e-19, 1e19, 1e30, 3e38])
+def test_grad_norm_magnitudes(size):
+    from gaussianimage_amd.adamw import grad_norm
+    g = torch.full((1, 3), size, dtype=F32, device=DEV)
+    want = math.sqrt(3) * float(g[0, 0])
+    norm, coef = grad_norm([g], 1.0)
+    if want > torch.finfo(F32).max:
+        assert torch.isinf(norm) and coef == 0
+    else:
+        assert abs(float(norm) - want) <= 2 * O.u * want + 2.0 ** -149
+        assert abs(float(coef) - min(1.0, 1 / (want + 1e-6))) <= 5 * O.u
+
+
+@pytest.mark.gpu
+def test_grad_norm_special_values():
+    from gaussianimage_amd.adamw import grad_norm
+    z = torch.zeros(5, device=DEV)
+    norm, coef = grad_norm([z, z[:0]], 1.0)
+    assert norm == 0 and coef == 1
+    for x, n in ((float("inf"), float("inf")), (float("nan"), float("nan"))):
+        a = z.clone()
+        a[3] = x
+        norm, coef = grad_norm([z, a], 1.0)
+        assert (torch.isinf(norm) and coef == 0) if n == float("inf") else (torch.isnan(norm) and torch.isnan(coef))
+    norm, _ = grad_norm([z[:0]])
+    assert norm == 0
+
+
+# ------------------------------------------------------------------ GPU: bindings, streams, graphs
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_both_bindings_give_the_same_bits(bits):
+    from gaussianimage_amd import ops
+    out = []
+    for compiled in (True, False):
+        previous = ops.use_compiled(compiled)
+        c = Case([3, 700, 5000], BF16, F32, bits, True, seed=6)
+        versions = [x._version for x in c.cols["p"] + c.cols["m"] + c.cols["v"] + c.cols["w"]]
+        c.run(clip=torch.tensor(0.7, device=DEV))
+        ops.use_compiled(previous)
+        after = [x._version for x in c.cols["p"] + c.cols["m"] + c.cols["v"] + c.cols["w"]]
+        assert all(b > a for a, b in zip(versions, after))
+        out.append(c)
+    for k in ("p", "m", "v", "w", "sm", "sv"):
+        for a, b in zip(out[0].cols[k], out[1].cols[k]):
+            if a is not None:
+                assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.gpu
+def test_device_scalars_are_refused_when_they_do_not_fit(binding):
+    from gaussianimage_amd.adamw import adamw_step
+    c = Case([5], F32, F32, 32)
+    args = [c.cols[k] for k in ("p", "g", "m", "v")]
+    for kw in (dict(step=torch.tensor(1.0, device=DEV)), dict(step=torch.tensor(1)), dict(step=0),
+               dict(step=1, lr=torch.tensor([1e-3, 1e-3], device=DEV)),
+               dict(step=1, clip=torch.tensor(1.0)), dict(step=1, clip=torch.tensor(1.0, device=DEV).double())):
+        with pytest.raises(ValueError):
+            adamw_step(*args, **kw)
+    with pytest.raises(TypeError):
+        adamw_step(*args, step=1, clip=0.5)
+    c.check_guards()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_another_stream(bits):
+    """The step runs on the current stream, behind what was queued there."""
+    c = Case([300001], F32, F32, bits, seed=12)
+    keep = [g.clone() for g in c.cols["g"]]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        a = torch.randn(2048, 2048, device=DEV)
+        for _ in range(20):
+            a = a @ a * 1e-3
+        for g, k in zip(c.cols["g"], keep):
+            g.zero_()
+            g.add_(k)
+        c.run()
+    side.synchronize()
+    c.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_captured_steps(bits):
+    """Two optimizers captured into graphs of their own and replayed in turn, with eager work in
+    between and another learning rate from the third replay on, against eager steps."""
+    from gaussianimage_amd.adamw import AdamW
+    shapes = [(40, 30), (7,), (513,)]
+
+    def make(seed):
+        gen = torch.Generator().manual_seed(seed)
+        ps = [torch.nn.Parameter(torch.randn(s, generator=gen).to(DEV)) for s in shapes]
+        grads = [[torch.randn(s, generator=gen).to(DEV) for s in shapes] for _ in range(6)]
+        for p in ps:
+            p.grad = torch.zeros_like(p)
+        lr = torch.tensor(LR, device=DEV)
+        opt = AdamW(ps, lr=lr, max_grad_norm=1.0, state_bits=bits, capturable=True, seed=5)
+        return ps, grads, lr, opt
+
+    def feed(ps, grads, t):
+        for p, g in zip(ps, grads[t]):
+            p.grad.copy_(g)
+
+    runs = []
+    for seed in (1, 2):
+        ps, grads, lr, opt = make(seed)
+        feed(ps, grads, 0)
+        opt.step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            opt.step()
+        runs.append((ps, grads, lr, opt, graph))
+    want = [make(seed) for seed in (1, 2)]
+    for t in range(6):
+        for (ps, grads, lr, opt, graph), (qs, _, rate, eager) in zip(runs, want):
+            if t == 3:
+                lr.fill_(LR / 2)
+                rate.fill_(LR / 2)
+            feed(qs, grads, t)
+            eager.step()
+            if t > 0:
+                feed(ps, grads, t)
+                graph.replay()
+            torch.randn(100000, device=DEV).sum().item()
+            for p, q in zip(ps, qs):
+                assert torch.equal(p, q)
+                assert int(opt.state[p]["step"]) == t + 1
+
+
+@pytest.mark.gpu
+def test_capture_refusals():
+    from gaussianimage_amd.adamw import AdamW
+    p = torch.nn.Parameter(torch.zeros(10, device=DEV))
+    p.grad = torch.ones_like(p)
+    for opt, what in ((AdamW([p]), "capturable=True"), (AdamW([p], capturable=True), "before capturing")):
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match=what):
+            with torch.cuda.graph(graph):
+                torch.zeros(1, device=DEV)
+                opt.step()
+    q = torch.nn.Parameter(torch.zeros(10, device=DEV))
+    q.grad = torch.ones_like(q)
+    opt = AdamW([p, q], capturable=True)
+    opt.step()
+    q.grad = None
+    with pytest.raises(RuntimeError, match="together"):
+        opt.step()
+
+
+@pytest.mark.gpu
+def test_device_step_count_agrees_with_the_host():
+    """A step count and a learning rate in device memory: within the 2 units in the last place by
+    which the coefficients may differ (and the same 8-bit words)."""
+    from gaussianimage_amd.adamw import adamw_step, adamw_step_8bit
+    for bits in (32, 8):
+        for t in (1, 2, 1000, 123457):
+            a, b = (Case([5000], F32, F32, bits, seed=t) for _ in range(2))
+            a.run(t=t)
+            step, lr = torch.tensor([t], device=DEV), torch.tensor(LR, device=DEV)
+            b.run(t=step, lr=lr)
+            x, y = a.cols["p"][0].double(), b.cols["p"][0].double()
+            w = torch.tensor(a.np[0][0], device=DEV)
+            up = (x - w).abs()
+            assert torch.all((x - y).abs() <= O.u * (8 * up + 4 * x.abs()))
+            for k in ("m", "v"):
+                assert torch.equal(a.cols[k][0].view(torch.uint8), b.cols[k][0].view(torch.uint8))
+
+
+# ------------------------------------------------------------------ GPU: the optimizer
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("state_bits", [32, 8])
+@pytest.mark.parametrize("dtype,master", [(F32, False), (BF16, True), (F16, False)])
+def test_optimizer_follows_the_operators(dtype, master, state_bits, binding):
+    """Groups of their own hyperparameters, a parameter that joins late, one without gradients,
+    one whose gradient is broadcast, clipping over all of them."""
+    from gaussianimage_amd.adamw import AdamW
+    gen = torch.Generator().manual_seed(4)
+    shapes = [(300, 2), (300, 3), (5,), (17, 9), (4,)]
+    ps = [torch.nn.Parameter(torch.randn(s, generator=gen).to(DEV, dtype)) for s in shapes]
+    opt = AdamW([{"params": ps[:2], "lr": 1e-2}, {"params": ps[2:], "weight_decay": 0.1}], max_grad_norm=0.5,
+                state_bits=state_bits, master_weights=master, seed=9)
+    w = [p.detach().double().cpu().numpy() for p in ps]
+    steps = [0] * 5
+    for it in range(4):
+        for i, p in enumerate(ps):
+            p.grad = None
+            if i == 4 or (i == 3 and it < 2):
+                continue
+            p.grad = torch.randn(shapes[i], generator=gen).to(DEV, dtype)
+        ps[2].grad = torch.tensor(0.25, device=DEV, dtype=dtype).expand(5)
+        _, coef = O.grad_norm([p.grad.double().cpu().numpy() for p in ps if p.grad is not None], 0.5)
+        coef = np.float32(coef)
+        states = [{k: (v.clone() if torch.is_tensor(v) else v) for k, v in opt.state.get(p, {}).items()} for p in ps]
+        grads = [None if p.grad is None else p.grad.clone() for p in ps]
+        opt.step()
+        for i, p in enumerate(ps):
+            if grads[i] is None:
+                assert np.array_equal(p.detach().double().cpu().numpy(), w[i])
+                continue
+            assert torch.equal(p.grad, grads[i])
+            steps[i] += 1
+            st = states[i]
+            if not st:
+                m, v = np.zeros(shapes[i]), np.zeros(shapes[i])
+            elif state_bits == 32:
+                m, v = (st[k].double().cpu().numpy() for k in ("exp_avg", "exp_avg_sq"))
+            else:
+                m, v = (O.decode(st[k].view(torch.uint8).cpu().numpy().reshape(-1), st[k + "_scale"].cpu().numpy(),
+                                 p.numel()).reshape(shapes[i]) for k in ("exp_avg", "exp_avg_rms"))
+                v = v * v
+            lr, wd = (1e-2, DECAY) if i < 2 else (LR, 0.1)
+            new, _, _, tol, _, _ = O.step(w[i], grads[i].double().cpu().numpy(), m, v, steps[i], lr, BETAS, EPS, wd,
+                                          coef, more=6)  # the coefficient: 5, and its rounding here
+            if master:
+                _near(opt.state[p]["master"], new, tol, f"master {i}")
+                assert torch.equal(p, opt.state[p]["master"].to(dtype))
+                w[i] = opt.state[p]["master"].double().cpu().numpy()
+            else:
+                info = torch.finfo(dtype)
+                half = 0 if dtype == F32 else np.maximum(np.abs(new) * info.eps / 2, info.tiny * info.eps / 2)
+                _near(p, new, tol * (1 + info.eps) + half, f"parameter {i}")
+                w[i] = p.detach().double().cpu().numpy()
+            assert opt.state[p]["step"] == steps[i]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("capturable", [False, True])
+@pytest.mark.parametrize("state_bits", [32, 8])
+def test_state_dict_goes_on_with_the_same_bits(state_bits, capturable, tmp_path):
+    from gaussianimage_amd.adamw import AdamW
+    gen = torch.Generator().manual_seed(4)
+    shapes = [(300, 2), (70,), (3,)]
+    start = [torch.randn(s, generator=gen).to(DEV, BF16) for s in shapes]
+    grads = [[torch.randn(s, generator=gen).to(DEV, BF16) for s in shapes] for _ in range(4)]
+
+    def make():
+        ps = [torch.nn.Parameter(x.clone()) for x in start]
+        return ps, AdamW([{"params": ps[:1], "lr": 0.1}, {"params": ps[1:]}], state_bits=state_bits,
+                         master_weights=True, capturable=capturable, seed=3)
+
+    def run(ps, opt, its):
+        for t in its:
+            for p, g in zip(ps[:2], grads[t]):       # (the third one never has a gradient)
+                p.grad = g.clone()
+            opt.step()
+
+    ps, opt = make()
+    run(ps, opt, range(4))
+    qs, first = make()
+    run(qs, first, range(2))
+    torch.save(first.state_dict(), tmp_path / "state.pt")
+    held = [q.detach().clone() for q in qs]
+    rs, second = make()
+    with torch.no_grad():
+        for r, h in zip(rs, held):
+            r.copy_(h)
+    second.load_state_dict(torch.load(tmp_path / "state.pt", weights_only=True))
+    run(rs, second, range(2, 4))
+    for p, r in zip(ps, rs):
+        assert torch.equal(p, r)
+        assert set(opt.state.get(p, {})) == set(second.state.get(r, {}))
+        for k, x in opt.state.get(p, {}).items():
+            y = second.state[r][k]
+            assert (torch.equal(x.view(torch.uint8), y.view(torch.uint8)) and x.dtype == y.dtype) \
+                if torch.is_tensor(x) else x == y
+    with pytest.raises(ValueError, match="state_bits"):
+        AdamW(rs, state_bits=40 - state_bits).load_state_dict(first.state_dict())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("state_bits", [32, 8])
+def test_an_image_fit_with_clipped_adamw(state_bits):
+    """The operators as a fit uses them together: projection, rasteriser, loss, backward, norm,
+    step -- every step against the restatement from that step's own gradients."""
+    from gaussianimage_amd._testing import harness, synth
+    from gaussianimage_amd.adamw import AdamW
+    torch.manual_seed(0)
+    model = harness.CholeskyImageModel(700, 64, 96, DEV, passes=1)
+    model.optimizer = opt = AdamW(model.parameters(), lr=1e-2, max_grad_norm=1e-3, state_bits=state_bits)
+    gt = synth.target_image(64, 96).to(DEV)
+    ps = list(model.parameters())
+    seen = {}
+    whole_step = opt.step
+
+    def step():
+        seen["grads"] = [p.grad.double().cpu().numpy() for p in ps]
+        whole_step()
+    opt.step = step
+    m = [np.zeros(tuple(p.shape)) for p in ps]
+    v = [np.zeros(tuple(p.shape)) for p in ps]
+    for t in range(1, 5):
+        w = [p.detach().double().cpu().numpy() for p in ps]
+        model.train_iter(gt)
+        _, coef = O.grad_norm(seen["grads"], 1e-3)
+        for i, p in enumerate(ps):
+            new, _, _, tol, _, _ = O.step(w[i], seen["grads"][i], m[i], v[i], t, 1e-2, BETAS, EPS, DECAY,
+                                          np.float32(coef), more=6)
+            _near(p, new, tol, f"parameter {i}, step {t}")
+            st = opt.state[p]
+            if state_bits == 32:
+                m[i], v[i] = (st[k].double().cpu().numpy() for k in ("exp_avg", "exp_avg_sq"))
+            else:
+                m[i], r = (O.decode(st[k].view(torch.uint8).cpu().numpy().reshape(-1), st[k + "_scale"].cpu().numpy(),
+                                    p.numel()).reshape(tuple(p.shape)) for k in ("exp_avg", "exp_avg_rms"))
+                v[i] = r * r
