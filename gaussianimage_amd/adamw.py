@@ -2,8 +2,8 @@
 with its clip coefficient -- beside ``adan.Adan`` for fits and trainings that want Adam's update.
 
 ``AdamW`` is the optimizer; ``adamw_step``, ``adamw_step_8bit`` and ``grad_norm`` are the calls it
-makes, for programs that keep their states themselves.  One launch steps up to 64 tensors (48 with
-8-bit states) of the same types.  GPU only, like the rest of the package: tensors on the CPU raise.
+makes, for programs that keep their states themselves.  One launch steps up to 124 tensors (82
+with 8-bit states) of the same types.  GPU only, like the rest of the package: tensors on the CPU raise.
 """
 import ctypes
 
@@ -48,10 +48,9 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.
 
     Every tensor must be dense, and a parameter's gradient and states laid out as it is.
     """
-    _check_hyper("adamw_step", lr, betas, eps, weight_decay, 0)
     (ops._C if ops._USE_C else _ctypes_binding).adamw_step(
         "adamw_step", 32, params, grads, exp_avgs, exp_avg_sqs, None, None, masters, step, lr,
-        betas[0], betas[1], eps, weight_decay, 0, clip)
+        betas, eps, weight_decay, 0, clip)
 
 
 def adamw_step_8bit(params, grads, exp_avgs, exp_avg_scales, exp_avg_rms, exp_avg_rms_scales, *,
@@ -67,10 +66,9 @@ def adamw_step_8bit(params, grads, exp_avgs, exp_avg_scales, exp_avg_rms, exp_av
     by a hash of (``seed``, ``step``, block, element), so that the same call gives the same bits.
     A sqrt(v) that is not zero never becomes zero; infinities and NaN become the NaN code.
     """
-    _check_hyper("adamw_step_8bit", lr, betas, eps, weight_decay, seed)
     (ops._C if ops._USE_C else _ctypes_binding).adamw_step(
         "adamw_step_8bit", 8, params, grads, exp_avgs, exp_avg_rms, exp_avg_scales,
-        exp_avg_rms_scales, masters, step, lr, betas[0], betas[1], eps, weight_decay, seed, clip)
+        exp_avg_rms_scales, masters, step, lr, betas, eps, weight_decay, seed, clip)
 
 
 def zero_state_8bit(param):
@@ -125,7 +123,8 @@ class _ctypes_binding:
 
     @classmethod
     def adamw_step(cls, op, bits, params, grads, exp_avgs, exp_avg_sqs, scales, sq_scales, masters,
-                   step, lr, beta1, beta2, eps, weight_decay, seed, clip):
+                   step, lr, betas, eps, weight_decay, seed, clip):
+        _check_hyper(op, lr, betas, eps, weight_decay, seed)
         names = {"params": params, "grads": grads, "exp_avgs": exp_avgs,
                  "exp_avg_rms" if bits == 8 else "exp_avg_sqs": exp_avg_sqs}
         if bits == 8:
@@ -200,7 +199,7 @@ class _ctypes_binding:
                                "of the parameter's, on its device")
                 t.exp_avg_scale, t.exp_avg_sq_scale = ops._ptr(scales[i]), ops._ptr(sq_scales[i])
         ops._need_cuda(op, params[0])
-        h = _lib.AdamWHyper(beta1=beta1, beta2=beta2, eps=eps, weight_decay=weight_decay, seed=seed,
+        h = _lib.AdamWHyper(beta1=betas[0], beta2=betas[1], eps=eps, weight_decay=weight_decay, seed=seed,
                             state_bits=bits, step=1)
         with torch.cuda.device(device):
             if torch.is_tensor(step):

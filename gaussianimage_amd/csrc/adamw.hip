@@ -7,39 +7,127 @@
 // 28 bytes move per element in 32 bits, 16 with 8-bit states (10 with bf16 parameters), for ~15
 // operations: long lists are bound by memory, short ones by the launch.  So everything about an
 // element is done in one pass, and a list of tensors goes into few launches: the pointers of up
-// to 64 (48 in 8 bits) tensors travel in the kernel arguments -- nothing is staged in device
+// to 124 (82 in 8 bits) tensors travel in the kernel arguments -- nothing is staged in device
 // memory, so a call may be captured into a graph -- and a workgroup finds the tensor of its chunk
-// with one load per lane and one ballot over the tensors' first chunks.
+// with one load per lane and a ballot over the tensors' first chunks.
 #include "host.h"
 
 #define ADAMW_THREADS 256
 #define ADAMW_CHUNK 2048          // elements of a workgroup: 8 per lane, 8 blocks of 256
 #define ADAMW_MAX_NUMEL ((int64_t)1 << 34)
 #define ADAMW_MAX_CHUNKS (1 << 23)  // chunks of a launch: 256 lanes each, below 2^32 lanes
+#define STREAM_PAST_BYTES ((int64_t)128 << 20)  // (see load_vec)
 
+// What depends on the hyperparameters and the step count; the floats are one vector, so that a
+// kernel takes them from its arguments or from device memory behind one branch.
+typedef float float8 __attribute__((ext_vector_type(8)));
 struct AdamWScalars {
-    float b1, omb1, b2, omb2, eps, decay, step, inv_bc2;
+    float8 f;
     unsigned key;
 };
+#define H_B1(h) ((h).f[0])       // beta1
+#define H_OMB1(h) ((h).f[1])     // 1 - beta1
+#define H_B2(h) ((h).f[2])
+#define H_OMB2(h) ((h).f[3])
+#define H_EPS(h) ((h).f[4])
+#define H_DECAY(h) ((h).f[5])    // 1 - lr * weight_decay
+#define H_STEP(h) ((h).f[6])     // lr / (1 - beta1^t)
+#define H_INV_BC2(h) ((h).f[7])  // 1 / sqrt(1 - beta2^t)
 
-// (Fields of 4 and 8 bytes only.  A scalar load ignores the two low bits of EACH part of its
-// address; with an array of bytes beside the others the compiler split an index 8 k into a base
-// + k and an offset 7 k, whose sum alone is aligned: pointers came from the wrong place.)
-template <int BITS>
-struct AdamWTable {
-    static constexpr int N = BITS == 8 ? 48 : 64;
-    void *p[N];
-    const void *g[N];
-    void *m[N];
-    void *v[N];
-    float *w[N];                            // masters
-    float *sm[BITS == 8 ? N : 1], *sv[BITS == 8 ? N : 1];
-    long long numel[N];
-    int first[N];                           // first chunk of the tensor in this launch
-    unsigned block0[BITS == 8 ? N : 1];     // first block of the tensor in the whole call
-    int vec[N];                             // every pointer allows four elements per access
-    int count;
+__device__ __forceinline__ AdamWScalars scalars_of(const AdamWScalars &args, const AdamWScalars *dev)
+{
+    AdamWScalars h = args;
+    if (dev) {
+        h.f = dev->f;
+        h.key = dev->key;
+    }
+    return h;
+}
+
+// What a launch is told of each tensor, in 32-bit words: 32 bytes, 40 with a master, 48 and 56 with
+// 8-bit states -- as many tensors as 4 KB of kernel arguments hold (with plain pointers a list of
+// 257 small tensors took 5 launches of 7 us instead of 3).  Pointers are 48 bits: the lower 32 in a
+// word each, the upper 16 in pairs.  (Words only: a scalar load ignores the two low bits of EACH
+// part of its address, and with an array of bytes beside the others the compiler split an index
+// 8 k into a base + k and an offset 7 k, whose sum alone is aligned.)
+template <int BITS, bool MASTER>
+struct AdamWEntry {
+    unsigned p, g, m, v, pg, mv, numel;
 };
+template <>
+struct AdamWEntry<32, true> {
+    unsigned p, g, m, v, pg, mv, numel, w, w_hi;
+};
+template <>
+struct AdamWEntry<8, false> {
+    unsigned p, g, m, v, pg, mv, numel, sm, sv, ss, block0;
+};
+template <>
+struct AdamWEntry<8, true> {
+    unsigned p, g, m, v, pg, mv, numel, sm, sv, ss, block0, w, w_hi;
+};
+
+template <int BITS, bool MASTER>
+struct AdamWTable {
+    typedef AdamWEntry<BITS, MASTER> Entry;
+    static constexpr int N = 3968 / (sizeof(Entry) + 4);  // 124, 99, 82, 70
+    // bits 0 to 23: the tensor's first chunk in this launch (all ones behind the last tensor); 24 to
+    // 27: the upper bits of numel; 31: every pointer allows four elements per access
+    unsigned meta[N];
+    Entry e[N];
+};
+#define META_FIRST 0xffffffu
+#define META_VEC 0x80000000u
+
+template <typename T>
+__device__ __forceinline__ T *pointer48(unsigned lo, unsigned hi)
+{
+    // (by way of the global address space: accesses are global ones, not flat)
+    return (T *)(__attribute__((address_space(1))) T *)(((unsigned long long)(hi & 0xffffu) << 32) | lo);
+}
+
+template <int BITS, bool MASTER>
+struct AdamWView {  // one entry, taken apart
+    void *p;
+    const void *g;
+    void *m, *v;
+    float *w = nullptr, *sm = nullptr, *sv = nullptr;
+    long long n;
+    int chunk;        // of the tensor
+    unsigned block0 = 0;
+    bool vec;
+};
+
+// The tensor this workgroup's chunk belongs to: the last one whose first chunk is not behind it
+// (a tensor without elements is not in the table, so the first chunks rise).
+template <int BITS, bool MASTER>
+__device__ __forceinline__ AdamWView<BITS, MASTER> tensor_of(const AdamWTable<BITS, MASTER> &T)
+{
+    constexpr int N = AdamWTable<BITS, MASTER>::N;
+    static_assert(N > WAVE && N <= 2 * WAVE, "two ballots");
+    const int lane = threadIdx.x & (WAVE - 1);
+    const unsigned b = blockIdx.x;
+    const unsigned f0 = T.meta[lane] & META_FIRST;
+    const unsigned f1 = T.meta[lane + WAVE < N ? lane + WAVE : N - 1] & META_FIRST;
+    const int k = __popcll(__ballot(f0 <= b)) + __popcll(__ballot(f1 <= b && lane + WAVE < N)) - 1;
+    const AdamWEntry<BITS, MASTER> e = T.e[k];
+    const unsigned meta = T.meta[k];
+    AdamWView<BITS, MASTER> t;
+    t.p = pointer48<void>(e.p, e.pg);
+    t.g = pointer48<const void>(e.g, e.pg >> 16);
+    t.m = pointer48<void>(e.m, e.mv);
+    t.v = pointer48<void>(e.v, e.mv >> 16);
+    t.n = ((long long)(meta >> 24 & 15) << 32) | e.numel;
+    t.chunk = (int)(b - (meta & META_FIRST));
+    t.vec = (meta & META_VEC) != 0;
+    if constexpr (MASTER) t.w = pointer48<float>(e.w, e.w_hi);
+    if constexpr (BITS == 8) {
+        t.sm = pointer48<float>(e.sm, e.ss);
+        t.sv = pointer48<float>(e.sv, e.ss >> 16);
+        t.block0 = e.block0;
+    }
+    return t;
+}
 
 // ---- element types ---------------------------------------------------------------------------
 // Half types are widened exactly on the way in and rounded once, to nearest even, on the way out.
@@ -57,105 +145,146 @@ template <> struct Elem<GI2D_F16> {
     typedef _Float16 vec __attribute__((ext_vector_type(4)));
 };
 
-template <int TYPE>
-__device__ __forceinline__ void load4(const void *base, long long i, float *x)
+// NT: past the caches.  A call that touches more than the 256 MB of the last-level cache finds
+// nothing there and leaves nothing there: streamed, 200 M fp32 elements took 979 us instead of 1047,
+// 120 M with 8-bit states 327 instead of 361.  A smaller one finds its states again: 5.8 M elements
+// 25.0 us through the caches, 26.8 streamed (12 M: 49 and 55, but 65 and 56 when something else ran
+// in between).  The host chooses by the size of the call, at half the cache.
+template <bool NT, typename V>
+__device__ __forceinline__ V load_vec(const V *p)
 {
-    const typename Elem<TYPE>::vec q =
-        *(const typename Elem<TYPE>::vec *)((const typename Elem<TYPE>::type *)base + i);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = (float)q[j];
+    if constexpr (NT) return __builtin_nontemporal_load(p);
+    else return *p;
 }
 
+template <bool NT, typename V>
+__device__ __forceinline__ void store_vec(V *p, V x)
+{
+    if constexpr (NT) __builtin_nontemporal_store(x, p);
+    else *p = x;
+}
+
+// Four neighbouring elements as they lie in memory.  Loads stay apart from the conversions: what
+// is loaded for a chunk is all under way before anything waits.
 template <int TYPE>
+struct Four {
+    typedef typename Elem<TYPE>::type E;
+    typedef typename Elem<TYPE>::vec V;
+    V q;
+    // `i`: the group's first element; a group that does not lie wholly inside reads the first group
+    // of the tensor instead (n >= 4)
+    template <bool NT>
+    __device__ __forceinline__ void load(const void *base, long long i, bool whole)
+    {
+        q = load_vec<NT>((const V *)((const E *)base + (whole ? i : 0)));
+    }
+    // element by element; what is outside reads the last element
+    __device__ __forceinline__ void load_each(const void *base, long long i, long long n)
+    {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) q[j] = ((const E *)base)[i + j < n ? i + j : n - 1];
+    }
+    __device__ __forceinline__ void get(float *x) const
+    {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = (float)q[j];
+    }
+};
+
+template <int TYPE, bool NT>
 __device__ __forceinline__ void store4(void *base, long long i, const float *x)
 {
-    typename Elem<TYPE>::vec q;
+    typedef typename Elem<TYPE>::vec V;
+    V q;
 #pragma unroll
     for (int j = 0; j < 4; ++j) q[j] = (typename Elem<TYPE>::type)x[j];
-    *(typename Elem<TYPE>::vec *)((typename Elem<TYPE>::type *)base + i) = q;
+    store_vec<NT>((V *)((typename Elem<TYPE>::type *)base + i), q);
 }
 
 template <int TYPE>
-__device__ __forceinline__ float load1(const void *base, long long i)
+__device__ __forceinline__ void store_each(void *base, long long i, long long n, const float *x)
 {
-    return (float)((const typename Elem<TYPE>::type *)base)[i];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (i + j < n) ((typename Elem<TYPE>::type *)base)[i + j] = (typename Elem<TYPE>::type)x[j];
 }
 
-template <int TYPE>
-__device__ __forceinline__ void store1(void *base, long long i, float x)
+// One element; m and v are the new ones afterwards.
+__device__ __forceinline__ void adamw_element(const AdamWScalars &h, float g, float &p, float &m,
+                                              float &v)
 {
-    ((typename Elem<TYPE>::type *)base)[i] = (typename Elem<TYPE>::type)x;
+    m = m * H_B1(h) + g * H_OMB1(h);
+    v = v * H_B2(h) + (g * g) * H_OMB2(h);
+    p = p * H_DECAY(h) - (m / (sqrtf(v) * H_INV_BC2(h) + H_EPS(h))) * H_STEP(h);
 }
 
-// One element; m and v are the new ones afterwards, the root of v is returned.
-__device__ __forceinline__ float adamw_element(const AdamWScalars &h, float g, float &p, float &m,
-                                               float &v)
-{
-    m = m * h.b1 + g * h.omb1;
-    v = v * h.b2 + (g * g) * h.omb2;
-    const float root = sqrtf(v);
-    p = p * h.decay - (m / (root * h.inv_bc2 + h.eps)) * h.step;
-    return root;
-}
-
-// The tensor a chunk belongs to: the last one whose first chunk is not behind it (a tensor
-// without elements is not in the table, so the first chunks rise).
-__device__ __forceinline__ int tensor_of(const int *first, int count, int chunk)
-{
-    const int lane = threadIdx.x & (WAVE - 1);
-    const int f = lane < count ? first[lane] : INT_MAX;
-    return __popcll(__ballot(f <= chunk)) - 1;
-}
-
-template <int PT, int GT, bool MASTER>
+template <int PT, int GT, bool MASTER, bool NT>
 __global__ __launch_bounds__(ADAMW_THREADS) void adamw_step_kernel(
-    AdamWTable<32> T, AdamWScalars ha, const AdamWScalars *__restrict__ h_dev,
+    AdamWTable<32, MASTER> T, AdamWScalars ha, const AdamWScalars *__restrict__ h_dev,
     const float *__restrict__ clip_dev)
 {
-    const int k = tensor_of(T.first, T.count, (int)blockIdx.x);
-    const AdamWScalars h = h_dev ? *h_dev : ha;
+    const auto t = tensor_of(T);
+    const AdamWScalars h = scalars_of(ha, h_dev);
     const float clip = clip_dev ? *clip_dev : 1.0f;
-    const long long n = T.numel[k];
-    const long long base = (long long)((int)blockIdx.x - T.first[k]) * ADAMW_CHUNK;
-    void *__restrict__ p = T.p[k];
-    const void *__restrict__ g = T.g[k];
-    float *__restrict__ m = (float *)T.m[k];
-    float *__restrict__ v = (float *)T.v[k];
-    float *__restrict__ w = T.w[k];
-    if (T.vec[k] && base + ADAMW_CHUNK <= n) {
-        float pv[2][4], gv[2][4], mv[2][4], vv[2][4];
-        const long long i0 = base + 4 * (int)threadIdx.x;
+    const long long n = t.n, base = (long long)t.chunk * ADAMW_CHUNK;
+    void *__restrict__ p = t.p;
+    const void *__restrict__ g = t.g;
+    void *__restrict__ m = t.m;
+    void *__restrict__ v = t.v;
+    void *__restrict__ w = t.w;
+    constexpr int WT = MASTER ? GI2D_F32 : PT;  // what is read and updated
+    const void *__restrict__ w_in = MASTER ? w : p;
+    Four<GT> gq[2];
+    Four<WT> wq[2];
+    Four<GI2D_F32> mq[2], vq[2];
+    const long long i0 = base + 4 * (int)threadIdx.x;
+    // Groups that lie inside load at once, those outside load anything; the one across the end of
+    // the tensor -- or every one of a tensor that allows single elements only -- then loads again,
+    // element by element.  (With all of a tensor's last chunk element by element, one load after
+    // the other, a launch took 2 us more.)
+    const bool groups = t.vec && n >= 4;
+    if (groups) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const long long i = i0 + u * (ADAMW_CHUNK / 2);
-            load4<GT>(g, i, gv[u]);
-            if (MASTER) load4<GI2D_F32>(w, i, pv[u]);
-            else load4<PT>(p, i, pv[u]);
-            load4<GI2D_F32>(m, i, mv[u]);
-            load4<GI2D_F32>(v, i, vv[u]);
+            const bool whole = i + 4 <= n;
+            gq[u].template load<NT>(g, i, whole);
+            wq[u].template load<NT>(w_in, i, whole);
+            mq[u].template load<NT>(m, i, whole);
+            vq[u].template load<NT>(v, i, whole);
         }
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const long long i = i0 + u * (ADAMW_CHUNK / 2);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                adamw_element(h, gv[u][j] * clip, pv[u][j], mv[u][j], vv[u][j]);
-            store4<PT>(p, i, pv[u]);
-            if (MASTER) store4<GI2D_F32>(w, i, pv[u]);
-            store4<GI2D_F32>(m, i, mv[u]);
-            store4<GI2D_F32>(v, i, vv[u]);
-        }
-        return;
     }
-    // the end of a tensor, or one whose pointers allow single elements only
-    const long long end = base + ADAMW_CHUNK < n ? base + ADAMW_CHUNK : n;
-    for (long long i = base + threadIdx.x; i < end; i += ADAMW_THREADS) {
-        float pi = MASTER ? w[i] : load1<PT>(p, i), mi = m[i], vi = v[i];
-        adamw_element(h, load1<GT>(g, i) * clip, pi, mi, vi);
-        store1<PT>(p, i, pi);
-        if (MASTER) w[i] = pi;
-        m[i] = mi;
-        v[i] = vi;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const long long i = i0 + u * (ADAMW_CHUNK / 2);
+        if (i < n && (!groups || i + 4 > n)) {
+            gq[u].load_each(g, i, n);
+            wq[u].load_each(w_in, i, n);
+            mq[u].load_each(m, i, n);
+            vq[u].load_each(v, i, n);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const long long i = i0 + u * (ADAMW_CHUNK / 2);
+        float gx[4], wx[4], mx[4], vx[4];
+        gq[u].get(gx);
+        wq[u].get(wx);
+        mq[u].get(mx);
+        vq[u].get(vx);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) adamw_element(h, gx[j] * clip, wx[j], mx[j], vx[j]);
+        if (groups && i + 4 <= n) {
+            store4<PT, NT>(p, i, wx);
+            if (MASTER) store4<GI2D_F32, NT>(w, i, wx);
+            store4<GI2D_F32, NT>(m, i, mx);
+            store4<GI2D_F32, NT>(v, i, vx);
+        } else if (i < n) {
+            store_each<PT>(p, i, n, wx);
+            if (MASTER) store_each<GI2D_F32>(w, i, n, wx);
+            store_each<GI2D_F32>(m, i, n, mx);
+            store_each<GI2D_F32>(v, i, n, vx);
+        }
     }
 }
 
@@ -201,17 +330,22 @@ __device__ __forceinline__ int scale_exponent(unsigned top)
     return k < -100 ? -100 : k > 119 ? 119 : k;
 }
 
-// e4m3 code of x / 2^k.  |x| 2^(-k-120) has, as a float, the code's exponent and fraction in its
-// upper bits -- e4m3's subnormals line up with fp32's, which this part does not flush -- so adding
-// 20 random bits below them and cutting rounds at random.  16 of them are random and the half of
-// their last place is set: the mean is kept to 2^-16 of a code's step.
+// e4m3 code of |x| / 2^k in bits 20 to 26.  |x| 2^(-k-120) has, as a float, the code's exponent and
+// fraction in its upper bits -- e4m3's subnormals line up with fp32's, which this part does not
+// flush -- so adding 20 random bits below them and cutting rounds at random.  16 of them are random
+// and the half of their last place is set: the mean is kept to 2^-16 of a code's step.  What is
+// below 448 * 2^k stays there: the code of 448 has no bits below it to carry.
 __device__ __forceinline__ unsigned encode_e4m3(float x, int k, unsigned random16)
 {
-    const unsigned y = __float_as_uint(ldexpf(fabsf(x), -k - 120));
-    unsigned c = (y + (random16 * 16u + 8u)) >> 20;
-    c = c < 126u ? c : 126u;
-    if (!(fabsf(x) <= 3.402823466e38f)) c = 127u;  // infinities and NaN: the NaN code
-    return c | ((__float_as_uint(x) >> 24) & 0x80u);
+    return __float_as_uint(ldexpf(fabsf(x), -k - 120)) + (random16 * 16u + 8u);
+}
+
+// The same for a block that holds infinities or NaN (the NaN code) or values beyond 448 * 2^119
+// (the largest code).
+__device__ __forceinline__ unsigned encode_e4m3_any(float x, int k, unsigned random16)
+{
+    const unsigned c = encode_e4m3(x, k, random16) >> 20;
+    return (fabsf(x) <= 3.402823466e38f ? c < 126u ? c : 126u : 127u) << 20;
 }
 
 __device__ __forceinline__ unsigned finite_bits(float x)
@@ -231,107 +365,200 @@ __device__ __forceinline__ void decode4(unsigned codes, float scale, float *x)
     x[3] = hi[1] * scale;
 }
 
+// Bits 20 to 26 of four words and the signs beside them, as four bytes.
+__device__ __forceinline__ unsigned pack_codes(const unsigned *c, const unsigned *sign)
+{
+    unsigned t[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) t[j] = ((c[j] << 4) & 0x7fffffffu) | (sign[j] & 0x80000000u);
+    const unsigned lo = __builtin_amdgcn_perm(t[1], t[0], 0x0c0c0703u);
+    const unsigned hi = __builtin_amdgcn_perm(t[3], t[2], 0x07030c0cu);
+    return lo | hi;
+}
+
+// four codes, element by element; 0 outside
+__device__ __forceinline__ unsigned load_codes(const unsigned char *base, long long i, long long n)
+{
+    unsigned c[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c[j] = base[i + j < n ? i + j : n - 1];
+    return c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
+}
+
+__device__ __forceinline__ void store_codes(unsigned char *base, long long i, long long n, unsigned c)
+{
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (i + j < n) base[i + j] = (unsigned char)(c >> (8 * j));
+}
+
+struct Codes8 {
+    unsigned m, r;     // four codes each
+    int km, kr;        // the block's exponents
+};
+
+// Four neighbouring elements of a lane, the wave holding their block: the update of p, and the new
+// codes.  ~50 instructions an element.  The root and the quotient are the hardware's, one unit in
+// the last place each (the correctly rounded ones took half the instructions of the kernel, and 10
+// bytes per element leave 266 cycles for 64 of them): a tenth of a millionth of the step.
+__device__ __forceinline__ Codes8 step8(const AdamWScalars &h, const float *g, float clip, float *p,
+                                        unsigned cm, unsigned cr, float sm, float sr, unsigned block)
+{
+    const int lane = threadIdx.x & (WAVE - 1);
+    float m[4], r[4];
+    decode4(cm, sm, m);
+    decode4(cr, sr, r);
+    unsigned am[4], ar[4];
+    bool tiny = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float gj = g[j] * clip;
+        m[j] = m[j] * H_B1(h) + gj * H_OMB1(h);
+        r[j] = (r[j] * r[j]) * H_B2(h) + (gj * gj) * H_OMB2(h);
+        tiny = tiny || __builtin_amdgcn_classf(r[j], 0x80);  // a positive subnormal
+    }
+    if (__any(tiny)) {  // (the instruction takes subnormals for zeros)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[j] = sqrtf(r[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[j] = __builtin_amdgcn_sqrtf(r[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float q = m[j] * __builtin_amdgcn_rcpf(r[j] * H_INV_BC2(h) + H_EPS(h));
+        p[j] = p[j] * H_DECAY(h) - q * H_STEP(h);
+        am[j] = __float_as_uint(m[j]) & 0x7fffffffu;
+        ar[j] = __float_as_uint(r[j]) & 0x7fffffffu;
+    }
+    const auto up = [](unsigned a, unsigned b) { return a > b ? a : b; };
+    unsigned top_m = wave_max_u32(up(up(am[0], am[1]), up(am[2], am[3])));
+    unsigned top_r = wave_max_u32(up(up(ar[0], ar[1]), up(ar[2], ar[3])));
+    const unsigned hb = hash32(h.key + block * HASH_STRIDE);
+    unsigned word[4], em[4], er[4], none[4] = {0, 0, 0, 0}, sign[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        word[j] = hash32(hb + (unsigned)(4 * lane + j) * HASH_STRIDE);
+        sign[j] = __float_as_uint(m[j]);
+    }
+    Codes8 out;
+    // 0x7f600000: 448 * 2^119
+    if (up(top_m, top_r) <= 0x7f600000u) {
+        out.km = scale_exponent(top_m);
+        out.kr = scale_exponent(top_r);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            em[j] = encode_e4m3(m[j], out.km, word[j] >> 16);
+            er[j] = encode_e4m3(r[j], out.kr, word[j] & 0xffffu);
+        }
+    } else {
+        out.km = scale_exponent(wave_max_u32(up(up(finite_bits(m[0]), finite_bits(m[1])),
+                                                up(finite_bits(m[2]), finite_bits(m[3])))));
+        out.kr = scale_exponent(wave_max_u32(up(up(finite_bits(r[0]), finite_bits(r[1])),
+                                                up(finite_bits(r[2]), finite_bits(r[3])))));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            em[j] = encode_e4m3_any(m[j], out.km, word[j] >> 16);
+            er[j] = encode_e4m3_any(r[j], out.kr, word[j] & 0xffffu);
+        }
+    }
+    // A root that is not zero stays so: with a mean beside it, the next step would divide by eps
+    // alone.  (The root of an fp32 number is 0 or above 2^-76: its bits are above 1 << 20.)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) er[j] = up(er[j], ar[j] < 0x100000u ? ar[j] : 0x100000u);
+    out.m = pack_codes(em, sign);
+    out.r = pack_codes(er, none);
+    return out;
+}
+
 // A wave owns whole blocks of 256 elements, four neighbouring ones per lane, so that a block's
-// largest magnitudes need no memory and its scale no atomics.
-template <int PT, int GT, bool MASTER>
+// largest magnitudes need no memory and its scale no atomics; two blocks, the loads of both ahead
+// of the arithmetic.
+template <int PT, int GT, bool MASTER, bool NT>
 __global__ __launch_bounds__(ADAMW_THREADS) void adamw_step8_kernel(
-    AdamWTable<8> T, AdamWScalars ha, const AdamWScalars *__restrict__ h_dev,
+    AdamWTable<8, MASTER> T, AdamWScalars ha, const AdamWScalars *__restrict__ h_dev,
     const float *__restrict__ clip_dev)
 {
-    const int k = tensor_of(T.first, T.count, (int)blockIdx.x);
-    const AdamWScalars h = h_dev ? *h_dev : ha;
+    const auto t = tensor_of(T);
+    const AdamWScalars h = scalars_of(ha, h_dev);
     const float clip = clip_dev ? *clip_dev : 1.0f;
-    const long long n = T.numel[k];
+    const long long n = t.n;
     const int lane = threadIdx.x & (WAVE - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-    const bool vec = T.vec[k];
-    void *__restrict__ p = T.p[k];
-    const void *__restrict__ g = T.g[k];
-    unsigned char *__restrict__ m = (unsigned char *)T.m[k];
-    unsigned char *__restrict__ v = (unsigned char *)T.v[k];
-    float *__restrict__ w = T.w[k];
-    float *__restrict__ sm = T.sm[k], *__restrict__ sv = T.sv[k];
-    const long long block = (long long)((int)blockIdx.x - T.first[k]) *
-                                (ADAMW_CHUNK / GI2D_ADAMW_BLOCK) + wave * 2;
-    float pv[2][4], gv[2][4], mv[2][4], vv[2][4], km[2], kv[2];
+    void *__restrict__ p = t.p;
+    const void *__restrict__ g = t.g;
+    unsigned char *__restrict__ m = (unsigned char *)t.m;
+    unsigned char *__restrict__ v = (unsigned char *)t.v;
+    void *__restrict__ w = t.w;
+    float *__restrict__ sm = t.sm, *__restrict__ sv = t.sv;
+    const long long block = (long long)t.chunk * (ADAMW_CHUNK / GI2D_ADAMW_BLOCK) + wave * 2;
+    const unsigned number = t.block0 + (unsigned)block;
+    const long long i0 = block * GI2D_ADAMW_BLOCK + 4 * lane;
+    const auto exponent_scale = [](int e) { return __uint_as_float((unsigned)(e + 127) << 23); };
+    if (block * GI2D_ADAMW_BLOCK >= n) return;
+    const bool second = (block + 1) * GI2D_ADAMW_BLOCK < n;
+    constexpr int WT = MASTER ? GI2D_F32 : PT;  // what is read and updated
+    const void *__restrict__ w_in = MASTER ? w : p;
+    Four<GT> gq[2];
+    Four<WT> wq[2];
     unsigned mc[2], vc[2];
-    bool whole[2], some[2];
+    float km[2], kv[2];
+    const bool groups = t.vec && n >= 4;  // (see adamw_step_kernel)
+    if (groups) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const long long b0 = (block + u) * GI2D_ADAMW_BLOCK, i = b0 + 4 * lane;
-        some[u] = b0 < n;
-        whole[u] = vec && b0 + GI2D_ADAMW_BLOCK <= n;
-        if (!some[u]) continue;
-        km[u] = sm[block + u];
-        kv[u] = sv[block + u];
-        if (whole[u]) {
-            load4<GT>(g, i, gv[u]);
-            if (MASTER) load4<GI2D_F32>(w, i, pv[u]);
-            else load4<PT>(p, i, pv[u]);
-            mc[u] = *(const unsigned *)(m + i);
-            vc[u] = *(const unsigned *)(v + i);
-        } else {
-            mc[u] = vc[u] = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                gv[u][j] = pv[u][j] = 0.0f;
-                if (i + j < n) {
-                    gv[u][j] = load1<GT>(g, i + j);
-                    pv[u][j] = MASTER ? w[i + j] : load1<PT>(p, i + j);
-                    mc[u] |= (unsigned)m[i + j] << (8 * j);
-                    vc[u] |= (unsigned)v[i + j] << (8 * j);
-                }
-            }
+        for (int u = 0; u < 2; ++u) {
+            const long long i = i0 + u * GI2D_ADAMW_BLOCK;
+            const bool whole = i + 4 <= n;
+            gq[u].template load<NT>(g, i, whole);
+            wq[u].template load<NT>(w_in, i, whole);
+            mc[u] = load_vec<NT>((const unsigned *)(m + (whole ? i : 0)));
+            vc[u] = load_vec<NT>((const unsigned *)(v + (whole ? i : 0)));
         }
     }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-        if (!some[u]) continue;
-        const long long i = (block + u) * GI2D_ADAMW_BLOCK + 4 * lane;
-        decode4(mc[u], km[u], mv[u]);
-        decode4(vc[u], kv[u], vv[u]);
-        float root[4];
-        unsigned top_m = 0, top_r = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            vv[u][j] = vv[u][j] * vv[u][j];
-            root[j] = adamw_element(h, gv[u][j] * clip, pv[u][j], mv[u][j], vv[u][j]);
-            const unsigned bm = finite_bits(mv[u][j]), br = finite_bits(root[j]);
-            top_m = top_m > bm ? top_m : bm;
-            top_r = top_r > br ? top_r : br;
+        km[u] = sm[block + (second ? u : 0)];
+        kv[u] = sv[block + (second ? u : 0)];
+        const long long i = i0 + u * GI2D_ADAMW_BLOCK;
+        if (i < n && (!groups || i + 4 > n)) {
+            gq[u].load_each(g, i, n);
+            wq[u].load_each(w_in, i, n);
+            mc[u] = load_codes(m, i, n);
+            vc[u] = load_codes(v, i, n);
         }
-        const int em = scale_exponent(wave_max_u32(top_m)), er = scale_exponent(wave_max_u32(top_r));
-        const unsigned hb = hash32(h.key + (T.block0[k] + (unsigned)(block + u)) * HASH_STRIDE);
-        unsigned cm = 0, cr = 0;
+    }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const unsigned r = hash32(hb + (unsigned)(4 * lane + j) * HASH_STRIDE);
-            const unsigned c = encode_e4m3(mv[u][j], em, r >> 16);
-            unsigned d = encode_e4m3(root[j], er, r & 0xffffu);
-            // a root that is not zero stays so: with a mean beside it, the next step would divide
-            // by eps alone
-            if (d == 0u && root[j] > 0.0f) d = 1u;
-            cm |= c << (8 * j);
-            cr |= d << (8 * j);
-        }
-        if (whole[u]) {
-            store4<PT>(p, i, pv[u]);
-            if (MASTER) store4<GI2D_F32>(w, i, pv[u]);
-            *(unsigned *)(m + i) = cm;
-            *(unsigned *)(v + i) = cr;
-        } else {
+    for (int u = 0; u < 2; ++u) {
+        if (u == 1 && !second) return;
+        const long long i = i0 + u * GI2D_ADAMW_BLOCK;
+        float gx[4], wx[4];
+        gq[u].get(gx);
+        wq[u].get(wx);
+        if ((block + u + 1) * GI2D_ADAMW_BLOCK > n) {
+            // outside the tensor: zeros, which are no block's largest
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (i + j < n) {
-                    store1<PT>(p, i + j, pv[u][j]);
-                    if (MASTER) w[i + j] = pv[u][j];
-                    m[i + j] = (unsigned char)(cm >> (8 * j));
-                    v[i + j] = (unsigned char)(cr >> (8 * j));
+                if (i + j >= n) {
+                    gx[j] = 0.0f;
+                    mc[u] &= ~(255u << (8 * j));
+                    vc[u] &= ~(255u << (8 * j));
                 }
         }
+        const Codes8 c = step8(h, gx, clip, wx, mc[u], vc[u], km[u], kv[u], number + u);
+        if (groups && i + 4 <= n) {
+            store4<PT, NT>(p, i, wx);
+            if (MASTER) store4<GI2D_F32, NT>(w, i, wx);
+            store_vec<NT>((unsigned *)(m + i), c.m);
+            store_vec<NT>((unsigned *)(v + i), c.r);
+        } else if (i < n) {
+            store_each<PT>(p, i, n, wx);
+            if (MASTER) store_each<GI2D_F32>(w, i, n, wx);
+            store_codes(m, i, n, c.m);
+            store_codes(v, i, n, c.r);
+        }
         if (lane == 0) {
-            sm[block + u] = __uint_as_float((unsigned)(em + 127) << 23);
-            sv[block + u] = __uint_as_float((unsigned)(er + 127) << 23);
+            sm[block + u] = exponent_scale(c.km);
+            sv[block + u] = exponent_scale(c.kr);
         }
     }
 }
@@ -373,9 +600,9 @@ __global__ void adamw_scalars_kernel(AdamWScalars h, double beta1, double beta2,
         q1 = q1 * q1;
         q2 = q2 * q2;
     }
-    h.decay = (float)(1.0 - lr * weight_decay);
-    h.step = (float)lr / (float)(1.0 - p1);
-    h.inv_bc2 = 1.0f / sqrtf((float)(1.0 - p2));
+    H_DECAY(h) = (float)(1.0 - lr * weight_decay);
+    H_STEP(h) = (float)lr / (float)(1.0 - p1);
+    H_INV_BC2(h) = 1.0f / sqrtf((float)(1.0 - p2));
     *out = h;
 }
 
@@ -384,16 +611,23 @@ __global__ void adamw_scalars_kernel(AdamWScalars h, double beta1, double beta2,
 // is as exact as one of them) and leaves one partial; one workgroup adds the partials in a fixed
 // order: the same bits in every run, no atomics, no memory to clear.
 #define NORM_THREADS 256
-#define NORM_TENSORS 128
-#define NORM_CHUNK_BYTES 16384
+#define NORM_TENSORS 232
 #define NORM_GROUPS 2048
+#ifndef NORM_SMALL_BYTES
+#define NORM_SMALL_BYTES ((int64_t)32 << 20)
+#endif
+
+struct NormEntry {
+    unsigned g, numel;
+    // bits 0 to 15: the pointer's upper 16; 16, 17: element type; 18: single elements only; 24 to 27:
+    // the upper bits of numel
+    unsigned more;
+};
 
 struct NormTable {
-    const void *g[NORM_TENSORS];
-    long long numel[NORM_TENSORS];
-    int first[NORM_TENSORS];
-    int type[NORM_TENSORS];  // element type, + 4 where 16-byte loads are not allowed
-    int count, chunks;
+    int first[NORM_TENSORS];  // first chunk (INT_MAX behind the last tensor)
+    NormEntry e[NORM_TENSORS];
+    int chunks;
 };
 
 __device__ __forceinline__ void add_square(double &s, float x)
@@ -402,28 +636,43 @@ __device__ __forceinline__ void add_square(double &s, float x)
     s = s + d * d;
 }
 
-template <int TYPE>
+// LOADS of 16 bytes per lane are under way together.
+template <int TYPE, int LOADS>
 __device__ __forceinline__ void chunk_squares(const void *g, long long n, long long chunk, bool vec,
                                               double *s)
 {
-    constexpr int SIZE = TYPE == GI2D_F32 ? 4 : 2, V = 16 / SIZE, CHUNK = NORM_CHUNK_BYTES / SIZE;
+    constexpr int V = 16 / (TYPE == GI2D_F32 ? 4 : 2), CHUNK = NORM_THREADS * V * LOADS;
     typedef typename Elem<TYPE>::type E;
     typedef E vec_t __attribute__((ext_vector_type(V)));
     const long long base = chunk * CHUNK;
     const E *__restrict__ x = (const E *)g;
     if (vec && base + CHUNK <= n) {
-        vec_t q[4];
+        vec_t q[LOADS];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-            q[u] = *(const vec_t *)(x + base + (long long)(u * NORM_THREADS + (int)threadIdx.x) * V);
+        for (int u = 0; u < LOADS; ++u)
+            q[u] = load_vec<(LOADS > 2)>(
+                (const vec_t *)(x + base + (long long)(u * NORM_THREADS + (int)threadIdx.x) * V));
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < LOADS; ++u)
 #pragma unroll
             for (int j = 0; j < V; ++j) add_square(s[j & 3], (float)q[u][j]);
         return;
     }
-    const long long end = base + CHUNK < n ? base + CHUNK : n;
-    for (long long i = base + threadIdx.x; i < end; i += NORM_THREADS) add_square(s[0], (float)x[i]);
+    // the end of a tensor, or one that allows single elements only: eight loads at a time
+    for (int r = 0; r < CHUNK; r += 8 * NORM_THREADS) {
+        if (base + r >= n) break;
+        E y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const long long i = base + r + j * NORM_THREADS + (int)threadIdx.x;
+            y[j] = x[i < n ? i : n - 1];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const long long i = base + r + j * NORM_THREADS + (int)threadIdx.x;
+            add_square(s[j & 3], i < n ? (float)y[j] : 0.0f);
+        }
+    }
 }
 
 __device__ __forceinline__ double block_sum(double v, double *lds)
@@ -433,26 +682,32 @@ __device__ __forceinline__ double block_sum(double v, double *lds)
     if ((threadIdx.x & (WAVE - 1)) == 0) lds[threadIdx.x / WAVE] = v;
     __syncthreads();
     double t = 0.0;
-    for (int i = 0; i < (int)blockDim.x / WAVE; ++i) t = t + lds[i];
+#pragma unroll
+    for (int i = 0; i < NORM_THREADS / WAVE; ++i) t = t + lds[i];
     return t;
 }
 
+template <int LOADS>
 __global__ __launch_bounds__(NORM_THREADS) void grad_squares_kernel(NormTable T, double *partials)
 {
     __shared__ double lds[NORM_THREADS / WAVE];
     const int lane = threadIdx.x & (WAVE - 1);
-    const int f0 = lane < T.count ? T.first[lane] : INT_MAX;
-    const int f1 = lane + WAVE < T.count ? T.first[lane + WAVE] : INT_MAX;
+    static_assert(NORM_TENSORS > 3 * WAVE && NORM_TENSORS <= 4 * WAVE, "four ballots");
+    const int f0 = T.first[lane], f1 = T.first[lane + WAVE], f2 = T.first[lane + 2 * WAVE];
+    const bool in3 = lane + 3 * WAVE < NORM_TENSORS;
+    const int f3 = T.first[in3 ? lane + 3 * WAVE : NORM_TENSORS - 1];
     double s[4] = {0.0, 0.0, 0.0, 0.0};
     for (int c = (int)blockIdx.x; c < T.chunks; c += (int)gridDim.x) {
-        const int k = __popcll(__ballot(f0 <= c)) + __popcll(__ballot(f1 <= c)) - 1;
-        const int type = T.type[k];
-        const bool vec = type < 4;
-        const long long chunk = c - T.first[k], n = T.numel[k];
-        switch (type & 3) {
-            case GI2D_F32: chunk_squares<GI2D_F32>(T.g[k], n, chunk, vec, s); break;
-            case GI2D_BF16: chunk_squares<GI2D_BF16>(T.g[k], n, chunk, vec, s); break;
-            default: chunk_squares<GI2D_F16>(T.g[k], n, chunk, vec, s); break;
+        const int k = __popcll(__ballot(f0 <= c)) + __popcll(__ballot(f1 <= c)) +
+                      __popcll(__ballot(f2 <= c)) + __popcll(__ballot(f3 <= c && in3)) - 1;
+        const NormEntry e = T.e[k];
+        const void *g = pointer48<const void>(e.g, e.more);
+        const long long chunk = c - T.first[k], n = ((long long)(e.more >> 24 & 15) << 32) | e.numel;
+        const bool vec = !(e.more & 0x40000u);
+        switch (e.more >> 16 & 3) {
+            case GI2D_F32: chunk_squares<GI2D_F32, LOADS>(g, n, chunk, vec, s); break;
+            case GI2D_BF16: chunk_squares<GI2D_BF16, LOADS>(g, n, chunk, vec, s); break;
+            default: chunk_squares<GI2D_F16, LOADS>(g, n, chunk, vec, s); break;
         }
     }
     const double t = block_sum((s[0] + s[1]) + (s[2] + s[3]), lds);
@@ -461,12 +716,21 @@ __global__ __launch_bounds__(NORM_THREADS) void grad_squares_kernel(NormTable T,
 
 // out[0] = norm, out[1] = min(1, max_norm / (norm + 1e-6)).  The root in float of a sum brought
 // to [1/2, 2) by an even power of two: sums beyond fp32's range have norms within it.
-__global__ __launch_bounds__(1024) void grad_norm_kernel(const double *__restrict__ partials, int n,
-                                                         float max_norm, float *out)
+__global__ __launch_bounds__(NORM_THREADS) void grad_norm_kernel(const double *__restrict__ partials,
+                                                                 int n, float max_norm, float *out)
 {
-    __shared__ double lds[1024 / WAVE];
+    __shared__ double lds[NORM_THREADS / WAVE];
     double s = 0.0;
-    for (int i = threadIdx.x; i < n; i += (int)blockDim.x) s = s + partials[i];
+    for (int r = 0; r < n; r += 8 * NORM_THREADS) {
+        double y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int i = r + j * NORM_THREADS + (int)threadIdx.x;
+            y[j] = partials[i < n ? i : n - 1];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s = s + (r + j * NORM_THREADS + (int)threadIdx.x < n ? y[j] : 0.0);
+    }
     s = block_sum(s, lds);
     if (threadIdx.x != 0) return;
     float norm = (float)s;  // 0, infinity and NaN are their own roots
@@ -489,26 +753,101 @@ __global__ __launch_bounds__(1024) void grad_norm_kernel(const double *__restric
 // ------------------------------------------------------------------------------------------
 
 static bool type_ok(int t) { return t == GI2D_F32 || t == GI2D_BF16 || t == GI2D_F16; }
-static int type_size(int t) { return t == GI2D_F32 ? 4 : 2; }
+static constexpr int type_size(int t) { return t == GI2D_F32 ? 4 : 2; }
 static bool aligned(const void *p, int to) { return ((uintptr_t)p & (uintptr_t)(to - 1)) == 0; }
 
 template <int BITS, int PT, int GT, bool MASTER>
-static void adamw_launch(const AdamWTable<BITS> &T, int chunks, const AdamWScalars &h,
-                         const AdamWScalars *h_dev, const float *clip, hipStream_t st)
+static void adamw_launch(const AdamWTable<BITS, MASTER> &T, int chunks, bool stream_past,
+                         const AdamWScalars &h, const AdamWScalars *h_dev, const float *clip,
+                         hipStream_t st)
 {
-    if constexpr (BITS == 8)
-        adamw_step8_kernel<PT, GT, MASTER><<<dim3((unsigned)chunks), ADAMW_THREADS, 0, st>>>(T, h, h_dev, clip);
-    else
-        adamw_step_kernel<PT, GT, MASTER><<<dim3((unsigned)chunks), ADAMW_THREADS, 0, st>>>(T, h, h_dev, clip);
+    const dim3 grid((unsigned)chunks);
+    if constexpr (BITS == 8) {
+        if (stream_past)
+            adamw_step8_kernel<PT, GT, MASTER, true><<<grid, ADAMW_THREADS, 0, st>>>(T, h, h_dev, clip);
+        else
+            adamw_step8_kernel<PT, GT, MASTER, false><<<grid, ADAMW_THREADS, 0, st>>>(T, h, h_dev, clip);
+    } else {
+        if (stream_past)
+            adamw_step_kernel<PT, GT, MASTER, true><<<grid, ADAMW_THREADS, 0, st>>>(T, h, h_dev, clip);
+        else
+            adamw_step_kernel<PT, GT, MASTER, false><<<grid, ADAMW_THREADS, 0, st>>>(T, h, h_dev, clip);
+    }
+}
+
+static unsigned low32(const void *p) { return (unsigned)(uintptr_t)p; }
+static unsigned high16(const void *lo, const void *hi)
+{
+    return (unsigned)((uintptr_t)lo >> 32) | (unsigned)((uintptr_t)hi >> 32) << 16;
+}
+static bool has_48_bits(const void *p) { return ((uintptr_t)p >> 48) == 0; }
+
+// The tensors of one (parameter type, gradient type, masters or not), in tables of N.
+template <int BITS, int PT, int GT, bool MASTER>
+static int adamw_run(int num_tensors, const gi2d_adamw_tensor *ts, bool stream_past,
+                     const AdamWScalars &h, const AdamWScalars *h_dev, const float *clip,
+                     hipStream_t st)
+{
+    constexpr int N = AdamWTable<BITS, MASTER>::N;
+    AdamWTable<BITS, MASTER> T;
+    int count = 0, chunks = 0;
+    unsigned block0 = 0;
+    const auto flush = [&]() {
+        if (count == 0) return GI2D_OK;
+        for (int c = count; c < N; ++c) T.meta[c] = META_FIRST;
+        adamw_launch<BITS, PT, GT, MASTER>(T, chunks, stream_past, h, h_dev, clip, st);
+        count = chunks = 0;
+        return launch_status();
+    };
+    for (int i = 0; i < num_tensors; ++i) {
+        const gi2d_adamw_tensor &t = ts[i];
+        const unsigned at = block0;
+        block0 += (unsigned)((t.numel + GI2D_ADAMW_BLOCK - 1) / GI2D_ADAMW_BLOCK);
+        if (t.numel == 0 || t.param_type != PT || t.grad_type != GT || (t.master != nullptr) != MASTER)
+            continue;
+        const int more = (int)((t.numel + ADAMW_CHUNK - 1) / ADAMW_CHUNK);
+        if (count == N || chunks + more > ADAMW_MAX_CHUNKS) {
+            const int rc = flush();
+            if (rc != GI2D_OK) return rc;
+        }
+        constexpr int state = BITS == 8 ? 4 : 16;
+        const bool vec = aligned(t.param, 4 * type_size(PT)) && aligned(t.grad, 4 * type_size(GT)) &&
+                         aligned(t.exp_avg, state) && aligned(t.exp_avg_sq, state) &&
+                         (!MASTER || aligned(t.master, 16));
+        T.meta[count] = (unsigned)chunks | (unsigned)(t.numel >> 32) << 24 | (vec ? META_VEC : 0u);
+        auto &e = T.e[count];
+        e.p = low32(t.param);
+        e.g = low32(t.grad);
+        e.m = low32(t.exp_avg);
+        e.v = low32(t.exp_avg_sq);
+        e.pg = high16(t.param, t.grad);
+        e.mv = high16(t.exp_avg, t.exp_avg_sq);
+        e.numel = (unsigned)t.numel;
+        if constexpr (MASTER) {
+            e.w = low32(t.master);
+            e.w_hi = high16(t.master, nullptr);
+        }
+        if constexpr (BITS == 8) {
+            e.sm = low32(t.exp_avg_scale);
+            e.sv = low32(t.exp_avg_sq_scale);
+            e.ss = high16(t.exp_avg_scale, t.exp_avg_sq_scale);
+            e.block0 = at;
+        }
+        ++count;
+        chunks += more;
+    }
+    return flush();
 }
 
 template <int BITS>
-static void adamw_dispatch(int pt, int gt, bool master, const AdamWTable<BITS> &T, int chunks,
-                           const AdamWScalars &h, const AdamWScalars *h_dev, const float *clip,
-                           hipStream_t st)
+static int adamw_types(unsigned present, int num_tensors, const gi2d_adamw_tensor *ts,
+                       bool stream_past, const AdamWScalars &h, const AdamWScalars *h_dev,
+                       const float *clip, hipStream_t st)
 {
-#define ADAMW_CASE(P, G, M) \
-    if (pt == P && gt == G && master == M) return adamw_launch<BITS, P, G, M>(T, chunks, h, h_dev, clip, st)
+    int rc = GI2D_OK;
+#define ADAMW_CASE(P, G, M)                                                   \
+    if (rc == GI2D_OK && (present & (1u << (P * 6 + G * 2 + (M ? 1 : 0)))))   \
+        rc = adamw_run<BITS, P, G, M>(num_tensors, ts, stream_past, h, h_dev, clip, st)
 #define ADAMW_GRADS(P, M)           \
     ADAMW_CASE(P, GI2D_F32, M);     \
     ADAMW_CASE(P, GI2D_BF16, M);    \
@@ -520,57 +859,7 @@ static void adamw_dispatch(int pt, int gt, bool master, const AdamWTable<BITS> &
     ADAMW_GRADS(GI2D_F16, true);
 #undef ADAMW_GRADS
 #undef ADAMW_CASE
-}
-
-// The tensors of one (parameter type, gradient type, masters or not), in tables of N.
-template <int BITS>
-static int adamw_run(int num_tensors, const gi2d_adamw_tensor *ts, int pt, int gt, bool master,
-                     const AdamWScalars &h, const AdamWScalars *h_dev, const float *clip,
-                     hipStream_t st)
-{
-    AdamWTable<BITS> T;
-    T.count = 0;
-    int chunks = 0;
-    unsigned block0 = 0;
-    const auto flush = [&]() {
-        if (T.count == 0) return GI2D_OK;
-        adamw_dispatch<BITS>(pt, gt, master, T, chunks, h, h_dev, clip, st);
-        T.count = 0;
-        chunks = 0;
-        return launch_status();
-    };
-    for (int i = 0; i < num_tensors; ++i) {
-        const gi2d_adamw_tensor &t = ts[i];
-        const unsigned blocks = (unsigned)((t.numel + GI2D_ADAMW_BLOCK - 1) / GI2D_ADAMW_BLOCK);
-        const unsigned at = block0;
-        block0 += blocks;
-        if (t.numel == 0 || t.param_type != pt || t.grad_type != gt || (t.master != nullptr) != master)
-            continue;
-        const int more = (int)((t.numel + ADAMW_CHUNK - 1) / ADAMW_CHUNK);
-        if (T.count == AdamWTable<BITS>::N || chunks + more > ADAMW_MAX_CHUNKS) {
-            const int rc = flush();
-            if (rc != GI2D_OK) return rc;
-        }
-        const int c = T.count++;
-        T.p[c] = t.param;
-        T.g[c] = t.grad;
-        T.m[c] = t.exp_avg;
-        T.v[c] = t.exp_avg_sq;
-        T.w[c] = t.master;
-        T.numel[c] = t.numel;
-        T.first[c] = chunks;
-        const int state = BITS == 8 ? 4 : 16;
-        T.vec[c] = aligned(t.param, 4 * type_size(pt)) && aligned(t.grad, 4 * type_size(gt)) &&
-                   aligned(t.exp_avg, state) && aligned(t.exp_avg_sq, state) &&
-                   (!master || aligned(t.master, 16));
-        if constexpr (BITS == 8) {
-            T.sm[c] = t.exp_avg_scale;
-            T.sv[c] = t.exp_avg_sq_scale;
-            T.block0[c] = at;
-        }
-        chunks += more;
-    }
-    return flush();
+    return rc;
 }
 
 extern "C" {
@@ -586,6 +875,7 @@ int gi2d_adamw_step(int num_tensors, const gi2d_adamw_tensor *tensors,
         return GI2D_E_INVALID;
     const bool bits8 = hyper->state_bits == 8;
     unsigned present = 0;  // one bit per (parameter type, gradient type, masters)
+    int64_t bytes = 0;     // of memory the call touches
     for (int i = 0; i < num_tensors; ++i) {
         const gi2d_adamw_tensor &t = tensors[i];
         if (!type_ok(t.param_type) || !type_ok(t.grad_type) || t.numel < 0 ||
@@ -595,17 +885,23 @@ int gi2d_adamw_step(int num_tensors, const gi2d_adamw_tensor *tensors,
         if (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq) return GI2D_E_INVALID;
         if (bits8 && (!t.exp_avg_scale || !t.exp_avg_sq_scale)) return GI2D_E_INVALID;
         if (t.master && t.param_type == GI2D_F32) return GI2D_E_INVALID;
+        const void *const all[] = {t.param, t.grad, t.exp_avg, t.exp_avg_sq, t.exp_avg_scale,
+                                   t.exp_avg_sq_scale, t.master};
+        for (const void *x : all)
+            if (!has_48_bits(x)) return GI2D_E_INVALID;
+        bytes += t.numel * (type_size(t.param_type) + type_size(t.grad_type) + (bits8 ? 2 : 8) +
+                            (t.master ? 4 : 0));
         present |= 1u << (t.param_type * 6 + t.grad_type * 2 + (t.master ? 1 : 0));
     }
     if (!present) return GI2D_OK;
     hipStream_t st = (hipStream_t)stream;
     AdamWScalars h;
-    h.b1 = (float)hyper->beta1;
-    h.omb1 = (float)(1.0 - hyper->beta1);
-    h.b2 = (float)hyper->beta2;
-    h.omb2 = (float)(1.0 - hyper->beta2);
-    h.eps = (float)hyper->eps;
-    h.decay = h.step = h.inv_bc2 = 0.0f;
+    H_B1(h) = (float)hyper->beta1;
+    H_OMB1(h) = (float)(1.0 - hyper->beta1);
+    H_B2(h) = (float)hyper->beta2;
+    H_OMB2(h) = (float)(1.0 - hyper->beta2);
+    H_EPS(h) = (float)hyper->eps;
+    H_DECAY(h) = H_STEP(h) = H_INV_BC2(h) = 0.0f;
     h.key = 0;
     const AdamWScalars *h_dev = nullptr;
     if (on_device) {
@@ -619,22 +915,14 @@ int gi2d_adamw_step(int num_tensors, const gi2d_adamw_tensor *tensors,
         h_dev = (const AdamWScalars *)hyper->scalars_dev;
     } else {
         const double t = (double)hyper->step;
-        h.decay = (float)(1.0 - hyper->lr * hyper->weight_decay);
-        h.step = (float)(hyper->lr / (1.0 - pow(hyper->beta1, t)));
-        h.inv_bc2 = (float)(1.0 / sqrt(1.0 - pow(hyper->beta2, t)));
+        H_DECAY(h) = (float)(1.0 - hyper->lr * hyper->weight_decay);
+        H_STEP(h) = (float)(hyper->lr / (1.0 - pow(hyper->beta1, t)));
+        H_INV_BC2(h) = (float)(1.0 / sqrt(1.0 - pow(hyper->beta2, t)));
         h.key = step_key(hyper->seed, hyper->step);
     }
-    for (int pt = 0; pt < 3; ++pt)
-        for (int gt = 0; gt < 3; ++gt)
-            for (int master = 0; master < 2; ++master) {
-                if (!(present & (1u << (pt * 6 + gt * 2 + master)))) continue;
-                const int rc = bits8 ? adamw_run<8>(num_tensors, tensors, pt, gt, master != 0, h,
-                                                    h_dev, clip_dev, st)
-                                     : adamw_run<32>(num_tensors, tensors, pt, gt, master != 0, h,
-                                                     h_dev, clip_dev, st);
-                if (rc != GI2D_OK) return rc;
-            }
-    return GI2D_OK;
+    const bool stream_past = bytes > STREAM_PAST_BYTES;
+    return bits8 ? adamw_types<8>(present, num_tensors, tensors, stream_past, h, h_dev, clip_dev, st)
+                 : adamw_types<32>(present, num_tensors, tensors, stream_past, h, h_dev, clip_dev, st);
 }
 
 int64_t gi2d_grad_norm_workspace(int num_tensors)
@@ -649,43 +937,51 @@ int gi2d_grad_norm(int num_tensors, const void *const *grads, const int64_t *num
 {
     if (num_tensors < 0 || !out || !workspace || !(max_norm >= 0.0)) return GI2D_E_INVALID;
     if (num_tensors > 0 && (!grads || !numel || !types)) return GI2D_E_INVALID;
-    for (int i = 0; i < num_tensors; ++i)
+    int64_t bytes = 0;
+    for (int i = 0; i < num_tensors; ++i) {
         if (!type_ok(types[i]) || numel[i] < 0 || numel[i] > ADAMW_MAX_NUMEL ||
-            (numel[i] > 0 && !grads[i]))
+            (numel[i] > 0 && !grads[i]) || !has_48_bits(grads[i]))
             return GI2D_E_INVALID;
+        bytes += numel[i] * type_size(types[i]);
+    }
+    const bool small = bytes <= NORM_SMALL_BYTES;
+    const int chunk_bytes = NORM_THREADS * 16 * (small ? 2 : 8);
     hipStream_t st = (hipStream_t)stream;
     double *partials = (double *)workspace;
     NormTable T;
-    T.count = T.chunks = 0;
-    int done = 0;
+    int count = 0, done = 0;
+    T.chunks = 0;
     const auto flush = [&]() {
-        if (T.count == 0) return GI2D_OK;
+        if (count == 0) return GI2D_OK;
+        for (int c = count; c < NORM_TENSORS; ++c) T.first[c] = INT_MAX;
         const int groups = T.chunks < NORM_GROUPS ? T.chunks : NORM_GROUPS;
-        grad_squares_kernel<<<dim3((unsigned)groups), NORM_THREADS, 0, st>>>(T, partials + done);
+        if (small)
+            grad_squares_kernel<2><<<dim3((unsigned)groups), NORM_THREADS, 0, st>>>(T, partials + done);
+        else
+            grad_squares_kernel<8><<<dim3((unsigned)groups), NORM_THREADS, 0, st>>>(T, partials + done);
         done += groups;
-        T.count = T.chunks = 0;
+        count = T.chunks = 0;
         return launch_status();
     };
     for (int i = 0; i < num_tensors; ++i) {
         if (numel[i] == 0) continue;
-        const int64_t chunk = NORM_CHUNK_BYTES / type_size(types[i]);
-        const int64_t more = (numel[i] + chunk - 1) / chunk;  // at most 2^22
-        // (a table is full at 128 tensors, 2^29 chunks)
-        if (T.count == NORM_TENSORS) {
+        const int64_t chunk = chunk_bytes / type_size(types[i]);
+        const int64_t more = (numel[i] + chunk - 1) / chunk;  // at most 2^21: 232 tensors below 2^31
+        if (count == NORM_TENSORS) {
             const int rc = flush();
             if (rc != GI2D_OK) return rc;
         }
-        const int c = T.count++;
-        T.g[c] = grads[i];
-        T.numel[c] = numel[i];
-        T.type[c] = types[i] + (aligned(grads[i], 16) ? 0 : 4);
-        T.first[c] = T.chunks;
+        T.first[count] = T.chunks;
+        T.e[count].g = low32(grads[i]);
+        T.e[count].numel = (unsigned)numel[i];
+        T.e[count].more = high16(grads[i], nullptr) | (unsigned)types[i] << 16 |
+                          (aligned(grads[i], 16) ? 0u : 0x40000u) | (unsigned)(numel[i] >> 32) << 24;
         T.chunks += (int)more;
+        ++count;
     }
     int rc = flush();
     if (rc != GI2D_OK) return rc;
-    const int threads = done <= 256 ? 256 : 1024;
-    grad_norm_kernel<<<1, threads, 0, st>>>(partials, done, (float)max_norm, out);
+    grad_norm_kernel<<<1, NORM_THREADS, 0, st>>>(partials, done, (float)max_norm, out);
     return launch_status();
 }
 

@@ -88,9 +88,9 @@ class Written {
     }
 };
 
-inline void written(const at::Tensor &t)
+inline void written(c10::TensorImpl *t)
 {
-    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    if (!t->is_inference()) t->bump_version();
 }
 
 inline const at::Tensor *device_scalar(const char *op, const char *name, const py::object &o,
@@ -103,11 +103,40 @@ inline const at::Tensor *device_scalar(const char *op, const char *name, const p
     return &t;
 }
 
+[[noreturn]] inline void refuse_value(const char *op, const char *name, const char *range, double got)
+{
+    std::ostringstream msg;
+    msg << op << ": " << name << " must be " << range << ", got " << got;
+    throw py::value_error(msg.str());
+}
+
 void step(const char *op, int bits, const py::object &params_, const py::object &grads_,
           const py::object &m_, const py::object &v_, const py::object &sm_, const py::object &sv_,
-          const py::object &masters_, const py::object &step_, const py::object &lr_, double beta1,
-          double beta2, double eps, double weight_decay, uint32_t seed, const py::object &clip_)
+          const py::object &masters_, const py::object &step_, const py::object &lr_,
+          const std::pair<double, double> &betas, double eps, double weight_decay, int64_t seed,
+          const py::object &clip_)
 {
+    gi2d_adamw_hyper h;
+    h.lr = 0.0;
+    if (!THPVariable_Check(lr_.ptr())) {
+        h.lr = lr_.cast<double>();
+        if (!(h.lr >= 0.0)) refuse_value(op, "lr", ">= 0", h.lr);
+    }
+    for (double b : {betas.first, betas.second})
+        if (!(b >= 0.0 && b < 1.0)) refuse_value(op, "betas", "in [0, 1)", b);
+    if (!(eps >= 0.0)) refuse_value(op, "eps", ">= 0", eps);
+    if (!(weight_decay >= 0.0)) refuse_value(op, "weight_decay", ">= 0", weight_decay);
+    if (seed < 0 || seed >> 32 != 0) refuse_value(op, "seed", "in [0, 2^32)", (double)seed);
+    h.beta1 = betas.first;
+    h.beta2 = betas.second;
+    h.eps = eps;
+    h.weight_decay = weight_decay;
+    h.seed = (uint32_t)seed;
+    h.state_bits = bits;
+    h.step = 1;
+    h.step_dev = nullptr;
+    h.lr_dev = nullptr;
+    h.scalars_dev = nullptr;
     const Tensors params(params_, "params"), grads(grads_, "grads"), m(m_, "exp_avgs"),
         v(v_, bits == 8 ? "exp_avg_rms" : "exp_avg_sqs"), sm(sm_, "exp_avg_scales"),
         sv(sv_, "exp_avg_rms_scales"), masters(masters_, "masters");
@@ -132,6 +161,8 @@ void step(const char *op, int bits, const py::object &params_, const py::object 
                                        : "must be a float32 tensor laid out as its parameter";
     const at::Device device = params.at(0)->device();
     std::vector<gi2d_adamw_tensor> ts((size_t)n);
+    std::vector<c10::TensorImpl *> out;  // what the call writes
+    out.reserve((size_t)n * 6);
     Written seen((size_t)n * 4);
     for (int64_t i = 0; i < n; ++i) {
         const at::Tensor &p = *params.at(i), &g = *grads.at(i), &mi = *m.at(i), &vi = *v.at(i);
@@ -171,6 +202,8 @@ void step(const char *op, int bits, const py::object &params_, const py::object 
             fresh = fresh && (t.numel == 0 || seen.add(t.master));
         }
         if (!fresh) refuse(op, "params", i, "or its state appears twice");
+        for (const at::Tensor *x : {&p, &mi, &vi}) out.push_back(x->unsafeGetTensorImpl());
+        if (w != nullptr) out.push_back(w->unsafeGetTensorImpl());
         if (bits == 8) {
             const at::Tensor &a = *sm.at(i), &b = *sv.at(i);
             const int64_t blocks = (t.numel + GI2D_ADAMW_BLOCK - 1) / GI2D_ADAMW_BLOCK;
@@ -180,6 +213,8 @@ void step(const char *op, int bits, const py::object &params_, const py::object 
                     refuse(op, x == &a ? sm.name : sv.name, i,
                            "must be a contiguous float32 tensor with one element for 256 of the "
                            "parameter's, on its device");
+            out.push_back(a.unsafeGetTensorImpl());
+            out.push_back(b.unsafeGetTensorImpl());
             if (t.numel) {
                 t.exp_avg_scale = a.data_ptr<float>();
                 t.exp_avg_sq_scale = b.data_ptr<float>();
@@ -187,18 +222,6 @@ void step(const char *op, int bits, const py::object &params_, const py::object 
         }
     }
     need_gpu(op, *params.at(0));
-    gi2d_adamw_hyper h;
-    h.beta1 = beta1;
-    h.beta2 = beta2;
-    h.eps = eps;
-    h.weight_decay = weight_decay;
-    h.seed = seed;
-    h.state_bits = bits;
-    h.step = 1;
-    h.lr = 0.0;
-    h.step_dev = nullptr;
-    h.lr_dev = nullptr;
-    h.scalars_dev = nullptr;
     const c10::DeviceGuard guard(device);
     if (THPVariable_Check(step_.ptr()))
         h.step_dev = device_scalar(op, "step", step_, at::kLong, device)->data_ptr<int64_t>();
@@ -207,8 +230,6 @@ void step(const char *op, int bits, const py::object &params_, const py::object 
     if (h.step < 1) throw py::value_error(std::string(op) + ": step counts from 1");
     if (THPVariable_Check(lr_.ptr()))
         h.lr_dev = device_scalar(op, "lr", lr_, at::kFloat, device)->data_ptr<float>();
-    else
-        h.lr = lr_.cast<double>();
     at::Tensor scalars;  // (goes back to the allocator of this stream behind the launch)
     if (h.step_dev != nullptr || h.lr_dev != nullptr) {
         scalars = at::empty({GI2D_ADAMW_SCALARS_BYTES}, at::TensorOptions().dtype(at::kByte).device(device));
@@ -223,16 +244,7 @@ void step(const char *op, int bits, const py::object &params_, const py::object 
     check(gi2d_adamw_step((int)n, ts.data(), &h, clip,
                           c10::hip::getCurrentHIPStream(device.index()).stream()),
           "gi2d_adamw_step", true);
-    for (int64_t i = 0; i < n; ++i) {
-        written(*params.at(i));
-        written(*m.at(i));
-        written(*v.at(i));
-        if (bits == 8) {
-            written(*sm.at(i));
-            written(*sv.at(i));
-        }
-        if (const at::Tensor *w = masters.at(i, true)) written(*w);
-    }
+    for (c10::TensorImpl *t : out) written(t);
 }
 
 py::tuple grad_norm(const py::object &grads_, double max_norm)
@@ -259,10 +271,12 @@ py::tuple grad_norm(const py::object &grads_, double max_norm)
     }
     need_gpu(op, *grads.at(0));
     const c10::DeviceGuard guard(device);
-    const at::Tensor work = at::empty({gi2d_grad_norm_workspace((int)n)},
-                                      at::TensorOptions().dtype(at::kByte).device(device));
+    // (goes back to the allocator of this stream behind the launches)
+    const c10::DataPtr work =
+        c10::GetAllocator(device.type())->allocate((size_t)gi2d_grad_norm_workspace((int)n));
+    const at::AutoDispatchBelowADInplaceOrView no_autograd;
     const at::Tensor out = at::empty({2}, at::TensorOptions().dtype(at::kFloat).device(device));
-    check(gi2d_grad_norm((int)n, ptr.data(), numel.data(), type.data(), max_norm, work.data_ptr(),
+    check(gi2d_grad_norm((int)n, ptr.data(), numel.data(), type.data(), max_norm, work.get(),
                          out.data_ptr<float>(), c10::hip::getCurrentHIPStream(device.index()).stream()),
           "gi2d_grad_norm", true);
     return py::make_tuple(out.select(0, 0), out.select(0, 1));

@@ -309,8 +309,8 @@ int gi2d_adan_step(int num_tensors, float *const *params, float *const *grads,
  *   p = p (1 - lr wd) - lr/(1-b1^t) * m / (sqrt(v)/sqrt(1-b2^t) + eps).
  * Parameters and gradients are fp32, bf16 or fp16, each tensor its own; arithmetic is fp32.  A half
  * parameter may have an fp32 master, which is then what is read and updated, the parameter its
- * rounding.  The gradients are not written.  One launch per 64 tensors (48 with 8-bit states) of
- * the same types; nothing is allocated and nothing is read on the host, so a call may be captured.
+ * rounding.  The gradients are not written.  One launch per 124 tensors of the
+ * same types (99 with masters, 82 with 8-bit states, 70 with both); nothing is allocated and nothing is read on the host, so a call may be captured.
  * No element may appear twice among what a call writes.
  * state_bits 32: exp_avg and exp_avg_sq are fp32.
  * state_bits 8: for GI2D_ADAMW_BLOCK consecutive elements one power-of-two scale and one e4m3 code

@@ -12,10 +12,13 @@ u = 2.0 ** -24
 BLOCK = 256
 
 
-def step(p, g, m, v, t, lr, betas, eps, weight_decay, clip=1.0, more=0):
+def step(p, g, m, v, t, lr, betas, eps, weight_decay, clip=1.0, more=0, bits=32):
     """New (p, m, v) and the bounds of their float32 counterparts.  Inputs are the float32 (or
     half) values, exactly; ``clip`` the float32 coefficient, ``more`` the roundings by which it may
-    itself be off."""
+    itself be off.  With 8-bit states the root and the reciprocal of the denominator are the
+    hardware's: a unit in the last place (2 roundings) each, instead of a correct root and quotient
+    (1 each), and the reciprocal is multiplied (1 more): 3 roundings more."""
+    hw = 3 if bits == 8 else 0
     p, g, m, v = (np.asarray(x, np.float64) for x in (p, g, m, v))
     b1, b2 = betas
     g = g * clip                                     # 1 rounding of g
@@ -33,7 +36,7 @@ def step(p, g, m, v, t, lr, betas, eps, weight_decay, clip=1.0, more=0):
         # denominator: half of v's 7, the root 1, the coefficient 1, the product 1, eps 1 and the
         # sum 1 = 8.5 (and `more`); the quotient 1, the step size 2, the product 1, the difference
         # 1: below 14
-        tol_p = u * (3 * np.abs(p) + (14 + more) * np.abs(up)) + step_size * tol_m / denom
+        tol_p = u * (3 * np.abs(p) + (14 + more + hw) * np.abs(up)) + step_size * tol_m / denom
     return p * (1 - lr * weight_decay) - up, m_new, v_new, tol_p, tol_m, tol_v
 
 
