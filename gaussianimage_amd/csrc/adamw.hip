@@ -13,7 +13,11 @@
 #include "host.h"
 
 #define ADAMW_THREADS 256
-#define ADAMW_CHUNK 2048          // elements of a workgroup: 8 per lane, 8 blocks of 256
+#define ADAMW_CHUNK 2048          // elements of a workgroup, 8 per lane
+#ifndef BLOCKS8
+#define BLOCKS8 4                 // blocks of 256 of a wave with 8-bit states
+#endif
+#define ADAMW_CHUNK8 (ADAMW_THREADS / WAVE * BLOCKS8 * GI2D_ADAMW_BLOCK)
 #define ADAMW_MAX_NUMEL ((int64_t)1 << 34)
 #define ADAMW_MAX_CHUNKS (1 << 23)  // chunks of a launch: 256 lanes each, below 2^32 lanes
 #define STREAM_PAST_BYTES ((int64_t)128 << 20)  // (see load_vec)
@@ -164,6 +168,14 @@ __device__ __forceinline__ void store_vec(V *p, V x)
     else *p = x;
 }
 
+// `bytes` into an array whose start is the same for a whole wave: such an address is a scalar base
+// and a 32-bit offset.
+template <typename T>
+__device__ __forceinline__ T *at(T *base, unsigned bytes)
+{
+    return (T *)((const char *)base + bytes);
+}
+
 // Four neighbouring elements as they lie in memory.  Loads stay apart from the conversions: what
 // is loaded for a chunk is all under way before anything waits.
 template <int TYPE>
@@ -171,18 +183,19 @@ struct Four {
     typedef typename Elem<TYPE>::type E;
     typedef typename Elem<TYPE>::vec V;
     V q;
-    // `i`: the group's first element; a group that does not lie wholly inside reads the first group
-    // of the tensor instead (n >= 4)
+    // `i`: the group's first element, from `base`; a group that does not lie wholly inside reads
+    // the first group instead (which does)
     template <bool NT>
-    __device__ __forceinline__ void load(const void *base, long long i, bool whole)
+    __device__ __forceinline__ void load(const void *base, unsigned i, bool whole)
     {
-        q = load_vec<NT>((const V *)((const E *)base + (whole ? i : 0)));
+        q = load_vec<NT>(at((const V *)base, (whole ? i : 0u) * (unsigned)sizeof(E)));
     }
     // element by element; what is outside reads the last element
-    __device__ __forceinline__ void load_each(const void *base, long long i, long long n)
+    __device__ __forceinline__ void load_each(const void *base, unsigned i, unsigned n)
     {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) q[j] = ((const E *)base)[i + j < n ? i + j : n - 1];
+        for (unsigned j = 0; j < 4; ++j)
+            q[j] = *at((const E *)base, (i + j < n ? i + j : n - 1) * (unsigned)sizeof(E));
     }
     __device__ __forceinline__ void get(float *x) const
     {
@@ -192,21 +205,29 @@ struct Four {
 };
 
 template <int TYPE, bool NT>
-__device__ __forceinline__ void store4(void *base, long long i, const float *x)
+__device__ __forceinline__ void store4(void *base, unsigned i, const float *x)
 {
     typedef typename Elem<TYPE>::vec V;
     V q;
 #pragma unroll
     for (int j = 0; j < 4; ++j) q[j] = (typename Elem<TYPE>::type)x[j];
-    store_vec<NT>((V *)((typename Elem<TYPE>::type *)base + i), q);
+    store_vec<NT>(at((V *)base, i * (unsigned)sizeof(typename Elem<TYPE>::type)), q);
 }
 
 template <int TYPE>
-__device__ __forceinline__ void store_each(void *base, long long i, long long n, const float *x)
+__device__ __forceinline__ void store_each(void *base, unsigned i, unsigned n, const float *x)
 {
+    typedef typename Elem<TYPE>::type E;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-        if (i + j < n) ((typename Elem<TYPE>::type *)base)[i + j] = (typename Elem<TYPE>::type)x[j];
+    for (unsigned j = 0; j < 4; ++j)
+        if (i + j < n) *at((E *)base, (i + j) * (unsigned)sizeof(E)) = (E)x[j];
+}
+
+// `elements` elements further on
+template <int TYPE>
+__device__ __forceinline__ void *further(const void *base, long long elements)
+{
+    return (typename Elem<TYPE>::type *)base + elements;
 }
 
 // One element; m and v are the new ones afterwards.
@@ -226,18 +247,18 @@ __global__ __launch_bounds__(ADAMW_THREADS) void adamw_step_kernel(
     const auto t = tensor_of(T);
     const AdamWScalars h = scalars_of(ha, h_dev);
     const float clip = clip_dev ? *clip_dev : 1.0f;
-    const long long n = t.n, base = (long long)t.chunk * ADAMW_CHUNK;
-    void *__restrict__ p = t.p;
-    const void *__restrict__ g = t.g;
-    void *__restrict__ m = t.m;
-    void *__restrict__ v = t.v;
-    void *__restrict__ w = t.w;
+    const long long base = (long long)t.chunk * ADAMW_CHUNK;
+    const unsigned n = t.n - base < ADAMW_CHUNK ? (unsigned)(t.n - base) : ADAMW_CHUNK;  // of this chunk
     constexpr int WT = MASTER ? GI2D_F32 : PT;  // what is read and updated
-    const void *__restrict__ w_in = MASTER ? w : p;
+    void *__restrict__ p = further<PT>(t.p, base);
+    const void *__restrict__ g = further<GT>(t.g, base);
+    void *__restrict__ m = further<GI2D_F32>(t.m, base);
+    void *__restrict__ v = further<GI2D_F32>(t.v, base);
+    void *__restrict__ w = MASTER ? further<GI2D_F32>(t.w, base) : p;
     Four<GT> gq[2];
     Four<WT> wq[2];
     Four<GI2D_F32> mq[2], vq[2];
-    const long long i0 = base + 4 * (int)threadIdx.x;
+    const unsigned i0 = 4 * threadIdx.x;
     // Groups that lie inside load at once, those outside load anything; the one across the end of
     // the tensor -- or every one of a tensor that allows single elements only -- then loads again,
     // element by element.  (With all of a tensor's last chunk element by element, one load after
@@ -246,27 +267,27 @@ __global__ __launch_bounds__(ADAMW_THREADS) void adamw_step_kernel(
     if (groups) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const long long i = i0 + u * (ADAMW_CHUNK / 2);
+            const unsigned i = i0 + u * (ADAMW_CHUNK / 2);
             const bool whole = i + 4 <= n;
             gq[u].template load<NT>(g, i, whole);
-            wq[u].template load<NT>(w_in, i, whole);
+            wq[u].template load<NT>(w, i, whole);
             mq[u].template load<NT>(m, i, whole);
             vq[u].template load<NT>(v, i, whole);
         }
     }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-        const long long i = i0 + u * (ADAMW_CHUNK / 2);
+        const unsigned i = i0 + u * (ADAMW_CHUNK / 2);
         if (i < n && (!groups || i + 4 > n)) {
             gq[u].load_each(g, i, n);
-            wq[u].load_each(w_in, i, n);
+            wq[u].load_each(w, i, n);
             mq[u].load_each(m, i, n);
             vq[u].load_each(v, i, n);
         }
     }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-        const long long i = i0 + u * (ADAMW_CHUNK / 2);
+        const unsigned i = i0 + u * (ADAMW_CHUNK / 2);
         float gx[4], wx[4], mx[4], vx[4];
         gq[u].get(gx);
         wq[u].get(wx);
@@ -308,18 +329,19 @@ __device__ __forceinline__ unsigned hash32(unsigned x)
 
 #define HASH_STRIDE 0x9E3779B9u  // odd: successive indices are far apart before they are hashed
 
-// Largest of the 64 lanes' values, in every lane (a lane's partners by row mirrors, as in
-// wave_sum_lane0).
+// Largest of the 64 lanes' values: within quads and rows, then lane 15 of rows 0 and 2 into rows 1
+// and 3, then lane 31 into rows 2 and 3 (as in wave_inclusive_scan); lane 63 has it.
 __device__ __forceinline__ unsigned wave_max_u32(unsigned v)
 {
+    // (a lane without a source receives 0)
     const auto up = [](unsigned a, int b) { return a > (unsigned)b ? a : (unsigned)b; };
     v = up(v, __builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, false));
     v = up(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, false));
     v = up(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, false));
     v = up(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xf, 0xf, false));
-    const unsigned r0 = __builtin_amdgcn_readlane((int)v, 0), r1 = __builtin_amdgcn_readlane((int)v, 16);
-    const unsigned r2 = __builtin_amdgcn_readlane((int)v, 32), r3 = __builtin_amdgcn_readlane((int)v, 48);
-    return up(up(r0, r1), up(r2, r3));
+    v = up(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false));
+    v = up(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false));
+    return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
 }
 
 // Exponent of the scale for a largest magnitude (its bits): 448 = 1.75 * 2^8.  At least 2^-100 (its
@@ -330,22 +352,24 @@ __device__ __forceinline__ int scale_exponent(unsigned top)
     return k < -100 ? -100 : k > 119 ? 119 : k;
 }
 
-// e4m3 code of |x| / 2^k in bits 20 to 26.  |x| 2^(-k-120) has, as a float, the code's exponent and
-// fraction in its upper bits -- e4m3's subnormals line up with fp32's, which this part does not
-// flush -- so adding 20 random bits below them and cutting rounds at random.  16 of them are random
+// e4m3 code of |x| / 2^k in bits 24 to 30.  |x| 2^(-k-120) has, as a float, the code's exponent and
+// fraction in its bits 20 to 26 -- e4m3's subnormals line up with fp32's, which this part does not
+// flush -- so adding random bits below them and cutting rounds at random.  16 of them are random
 // and the half of their last place is set: the mean is kept to 2^-16 of a code's step.  What is
 // below 448 * 2^k stays there: the code of 448 has no bits below it to carry.
-__device__ __forceinline__ unsigned encode_e4m3(float x, int k, unsigned random16)
+// `random`: in bits 8 to 23, bit 7 set.
+__device__ __forceinline__ unsigned encode_e4m3(float x, int k, unsigned random)
 {
-    return __float_as_uint(ldexpf(fabsf(x), -k - 120)) + (random16 * 16u + 8u);
+    return (__float_as_uint(ldexpf(fabsf(x), -k - 120)) << 4) + random;
 }
 
 // The same for a block that holds infinities or NaN (the NaN code) or values beyond 448 * 2^119
 // (the largest code).
-__device__ __forceinline__ unsigned encode_e4m3_any(float x, int k, unsigned random16)
+__device__ __forceinline__ unsigned encode_e4m3_any(float x, int k, unsigned random)
 {
-    const unsigned c = encode_e4m3(x, k, random16) >> 20;
-    return (fabsf(x) <= 3.402823466e38f ? c < 126u ? c : 126u : 127u) << 20;
+    if (!(fabsf(x) <= 3.402823466e38f)) return 127u << 24;
+    const unsigned y = __float_as_uint(ldexpf(fabsf(x), -k - 120));
+    return y >= 126u << 20 ? 126u << 24 : (y << 4) + random;
 }
 
 __device__ __forceinline__ unsigned finite_bits(float x)
@@ -354,41 +378,36 @@ __device__ __forceinline__ unsigned finite_bits(float x)
     return b < 0x7f800000u ? b : 0u;
 }
 
-__device__ __forceinline__ void decode4(unsigned codes, float scale, float *x)
+__device__ __forceinline__ void decode4(unsigned codes, float *x)
 {
     typedef float f2 __attribute__((ext_vector_type(2)));
     const f2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, false);
     const f2 hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, true);
-    x[0] = lo[0] * scale;
-    x[1] = lo[1] * scale;
-    x[2] = hi[0] * scale;
-    x[3] = hi[1] * scale;
+    x[0] = lo[0];
+    x[1] = lo[1];
+    x[2] = hi[0];
+    x[3] = hi[1];
 }
 
-// Bits 20 to 26 of four words and the signs beside them, as four bytes.
-__device__ __forceinline__ unsigned pack_codes(const unsigned *c, const unsigned *sign)
+// The upper bytes of four words.
+__device__ __forceinline__ unsigned pack_upper(const unsigned *t)
 {
-    unsigned t[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) t[j] = ((c[j] << 4) & 0x7fffffffu) | (sign[j] & 0x80000000u);
-    const unsigned lo = __builtin_amdgcn_perm(t[1], t[0], 0x0c0c0703u);
-    const unsigned hi = __builtin_amdgcn_perm(t[3], t[2], 0x07030c0cu);
-    return lo | hi;
+    return __builtin_amdgcn_perm(t[1], t[0], 0x0c0c0703u) | __builtin_amdgcn_perm(t[3], t[2], 0x07030c0cu);
 }
 
-// four codes, element by element; 0 outside
-__device__ __forceinline__ unsigned load_codes(const unsigned char *base, long long i, long long n)
+// four codes, element by element; what is outside reads the last one
+__device__ __forceinline__ unsigned load_codes(const unsigned char *base, unsigned i, unsigned n)
 {
     unsigned c[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) c[j] = base[i + j < n ? i + j : n - 1];
+    for (unsigned j = 0; j < 4; ++j) c[j] = base[i + j < n ? i + j : n - 1];
     return c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
 }
 
-__device__ __forceinline__ void store_codes(unsigned char *base, long long i, long long n, unsigned c)
+__device__ __forceinline__ void store_codes(unsigned char *base, unsigned i, unsigned n, unsigned c)
 {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (unsigned j = 0; j < 4; ++j)
         if (i + j < n) base[i + j] = (unsigned char)(c >> (8 * j));
 }
 
@@ -397,59 +416,88 @@ struct Codes8 {
     int km, kr;        // the block's exponents
 };
 
+// The factors of step8, the clip coefficient and the roots of those of the square folded in, and
+// the step size into the denominator.  (A step size of 0 makes the denominator's factors the
+// largest number: the quotient is 0.)
+struct Factors8 {
+    float b1, g_m, root_b2, g_r, decay, d_r, d_eps;
+    __device__ __forceinline__ Factors8(const AdamWScalars &h, float clip)
+    {
+        const float most = 3.402823466e38f;
+        b1 = H_B1(h);
+        g_m = H_OMB1(h) * clip;
+        root_b2 = sqrtf(H_B2(h));
+        g_r = sqrtf(H_OMB2(h)) * clip;
+        decay = H_DECAY(h);
+        d_r = fminf(H_INV_BC2(h) / H_STEP(h), most);
+        d_eps = fminf(H_EPS(h) / H_STEP(h), most);
+    }
+};
+
 // Four neighbouring elements of a lane, the wave holding their block: the update of p, and the new
-// codes.  ~50 instructions an element.  The root and the quotient are the hardware's, one unit in
-// the last place each (the correctly rounded ones took half the instructions of the kernel, and 10
-// bytes per element leave 266 cycles for 64 of them): a tenth of a millionth of the step.
-__device__ __forceinline__ Codes8 step8(const AdamWScalars &h, const float *g, float clip, float *p,
+// codes.  The root and the reciprocal are the hardware's, one unit in the last place each, and sums
+// of products are fused: a ten-millionth of the step.  (Correctly rounded root and quotient took
+// half the instructions of the kernel: 10 bytes per element leave 266 cycles for 64 of them, and an
+// instruction takes 4, before the instructions and not the memory set the time.)
+__device__ __forceinline__ Codes8 step8(const Factors8 &f, unsigned key, const float *g, float *p,
                                         unsigned cm, unsigned cr, float sm, float sr, unsigned block)
 {
     const int lane = threadIdx.x & (WAVE - 1);
     float m[4], r[4];
-    decode4(cm, sm, m);
-    decode4(cr, sr, r);
-    unsigned am[4], ar[4];
-    bool tiny = false;
+    decode4(cm, m);
+    decode4(cr, r);
+    const float m_b1 = sm * f.b1, r_b2 = sr * f.root_b2;  // (powers of two times the factors)
+    unsigned long long tiny = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const float gj = g[j] * clip;
-        m[j] = m[j] * H_B1(h) + gj * H_OMB1(h);
-        r[j] = (r[j] * r[j]) * H_B2(h) + (gj * gj) * H_OMB2(h);
-        tiny = tiny || __builtin_amdgcn_classf(r[j], 0x80);  // a positive subnormal
+        m[j] = __builtin_fmaf(m[j], m_b1, g[j] * f.g_m);
+        const float old = r[j] * r_b2, now = g[j] * f.g_r;
+        r[j] = __builtin_fmaf(old, old, now * now);
+        tiny |= __builtin_amdgcn_ballot_w64(__builtin_amdgcn_classf(r[j], 0x80));  // a positive subnormal
     }
-    if (__any(tiny)) {  // (the instruction takes subnormals for zeros)
+    if (tiny != 0) {  // (the instruction takes subnormals for zeros)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) r[j] = sqrtf(r[j]);
+        for (int j = 0; j < 4; ++j) {
+            const bool small = r[j] < 0x1p-64f;
+            const float root = __builtin_amdgcn_sqrtf(small ? r[j] * 0x1p64f : r[j]);
+            r[j] = small ? root * 0x1p-32f : root;
+        }
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) r[j] = __builtin_amdgcn_sqrtf(r[j]);
     }
+    unsigned ar[4];  // a root has no sign (a NaN may: it is above everything)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const float q = m[j] * __builtin_amdgcn_rcpf(r[j] * H_INV_BC2(h) + H_EPS(h));
-        p[j] = p[j] * H_DECAY(h) - q * H_STEP(h);
-        am[j] = __float_as_uint(m[j]) & 0x7fffffffu;
-        ar[j] = __float_as_uint(r[j]) & 0x7fffffffu;
+        const float quotient = __builtin_amdgcn_rcpf(__builtin_fmaf(r[j], f.d_r, f.d_eps));
+        p[j] = __builtin_fmaf(-m[j], quotient, p[j] * f.decay);
+        ar[j] = __float_as_uint(r[j]);
     }
     const auto up = [](unsigned a, unsigned b) { return a > b ? a : b; };
-    unsigned top_m = wave_max_u32(up(up(am[0], am[1]), up(am[2], am[3])));
-    unsigned top_r = wave_max_u32(up(up(ar[0], ar[1]), up(ar[2], ar[3])));
-    const unsigned hb = hash32(h.key + block * HASH_STRIDE);
-    unsigned word[4], em[4], er[4], none[4] = {0, 0, 0, 0}, sign[4];
+    // (fmaxf passes a NaN over)
+    const float am = fmaxf(fmaxf(fabsf(m[0]), fabsf(m[1])), fmaxf(fabsf(m[2]), fabsf(m[3])));
+    const unsigned top_m = wave_max_u32(__float_as_uint(am));
+    const unsigned top_r = wave_max_u32(up(up(ar[0], ar[1]), up(ar[2], ar[3])));
+    const bool strange = (__builtin_amdgcn_ballot_w64(__builtin_isunordered(m[0], m[1])) |
+                          __builtin_amdgcn_ballot_w64(__builtin_isunordered(m[2], m[3]))) != 0;
+    const unsigned hb = hash32(key + block * HASH_STRIDE);
+    unsigned word_m[4], word_r[4], em[4], er[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        word[j] = hash32(hb + (unsigned)(4 * lane + j) * HASH_STRIDE);
-        sign[j] = __float_as_uint(m[j]);
+        // the upper half of the element's word for the mean, the lower one for the root
+        const unsigned x = hash32(hb + (unsigned)(4 * lane + j) * HASH_STRIDE);
+        word_m[j] = __builtin_amdgcn_perm(x, 0x80u, 0x0c070600u);
+        word_r[j] = __builtin_amdgcn_perm(x, 0x80u, 0x0c050400u);
     }
     Codes8 out;
     // 0x7f600000: 448 * 2^119
-    if (up(top_m, top_r) <= 0x7f600000u) {
+    if (up(top_m, top_r) <= 0x7f600000u && !strange) {
         out.km = scale_exponent(top_m);
         out.kr = scale_exponent(top_r);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            em[j] = encode_e4m3(m[j], out.km, word[j] >> 16);
-            er[j] = encode_e4m3(r[j], out.kr, word[j] & 0xffffu);
+            em[j] = encode_e4m3(m[j], out.km, word_m[j]);
+            er[j] = encode_e4m3(r[j], out.kr, word_r[j]);
         }
     } else {
         out.km = scale_exponent(wave_max_u32(up(up(finite_bits(m[0]), finite_bits(m[1])),
@@ -458,22 +506,25 @@ __device__ __forceinline__ Codes8 step8(const AdamWScalars &h, const float *g, f
                                                 up(finite_bits(r[2]), finite_bits(r[3])))));
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            em[j] = encode_e4m3_any(m[j], out.km, word[j] >> 16);
-            er[j] = encode_e4m3_any(r[j], out.kr, word[j] & 0xffffu);
+            em[j] = encode_e4m3_any(m[j], out.km, word_m[j]);
+            er[j] = encode_e4m3_any(r[j], out.kr, word_r[j]);
         }
     }
     // A root that is not zero stays so: with a mean beside it, the next step would divide by eps
-    // alone.  (The root of an fp32 number is 0 or above 2^-76: its bits are above 1 << 20.)
+    // alone.  (The root of an fp32 number is 0 or above 2^-76: its bits are above 1 << 24.)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) er[j] = up(er[j], ar[j] < 0x100000u ? ar[j] : 0x100000u);
-    out.m = pack_codes(em, sign);
-    out.r = pack_codes(er, none);
+    for (int j = 0; j < 4; ++j) {
+        em[j] = (em[j] & 0x7fffffffu) | (__float_as_uint(m[j]) & 0x80000000u);
+        er[j] = up(er[j], ar[j] < 0x1000000u ? ar[j] : 0x1000000u);
+    }
+    out.m = pack_upper(em);
+    out.r = pack_upper(er);
     return out;
 }
 
 // A wave owns whole blocks of 256 elements, four neighbouring ones per lane, so that a block's
-// largest magnitudes need no memory and its scale no atomics; two blocks, the loads of both ahead
-// of the arithmetic.
+// largest magnitudes need no memory and its scale no atomics; the loads of all its blocks stand
+// ahead of the arithmetic.
 template <int PT, int GT, bool MASTER, bool NT>
 __global__ __launch_bounds__(ADAMW_THREADS) void adamw_step8_kernel(
     AdamWTable<8, MASTER> T, AdamWScalars ha, const AdamWScalars *__restrict__ h_dev,
@@ -482,59 +533,60 @@ __global__ __launch_bounds__(ADAMW_THREADS) void adamw_step8_kernel(
     const auto t = tensor_of(T);
     const AdamWScalars h = scalars_of(ha, h_dev);
     const float clip = clip_dev ? *clip_dev : 1.0f;
-    const long long n = t.n;
+    const Factors8 f(h, clip);
     const int lane = threadIdx.x & (WAVE - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-    void *__restrict__ p = t.p;
-    const void *__restrict__ g = t.g;
-    unsigned char *__restrict__ m = (unsigned char *)t.m;
-    unsigned char *__restrict__ v = (unsigned char *)t.v;
-    void *__restrict__ w = t.w;
-    float *__restrict__ sm = t.sm, *__restrict__ sv = t.sv;
-    const long long block = (long long)t.chunk * (ADAMW_CHUNK / GI2D_ADAMW_BLOCK) + wave * 2;
+    constexpr int OWN = BLOCKS8 * GI2D_ADAMW_BLOCK;  // elements of a wave
+    const long long block = (long long)t.chunk * (ADAMW_CHUNK8 / GI2D_ADAMW_BLOCK) + wave * BLOCKS8;
+    const long long base = block * GI2D_ADAMW_BLOCK;
+    if (base >= t.n) return;
+    const unsigned n = t.n - base < OWN ? (unsigned)(t.n - base) : OWN;  // of this wave
+    const int blocks = (int)(n + GI2D_ADAMW_BLOCK - 1) / GI2D_ADAMW_BLOCK;
     const unsigned number = t.block0 + (unsigned)block;
-    const long long i0 = block * GI2D_ADAMW_BLOCK + 4 * lane;
-    const auto exponent_scale = [](int e) { return __uint_as_float((unsigned)(e + 127) << 23); };
-    if (block * GI2D_ADAMW_BLOCK >= n) return;
-    const bool second = (block + 1) * GI2D_ADAMW_BLOCK < n;
     constexpr int WT = MASTER ? GI2D_F32 : PT;  // what is read and updated
-    const void *__restrict__ w_in = MASTER ? w : p;
-    Four<GT> gq[2];
-    Four<WT> wq[2];
-    unsigned mc[2], vc[2];
-    float km[2], kv[2];
+    void *__restrict__ p = further<PT>(t.p, base);
+    const void *__restrict__ g = further<GT>(t.g, base);
+    unsigned char *__restrict__ m = (unsigned char *)t.m + base;
+    unsigned char *__restrict__ v = (unsigned char *)t.v + base;
+    void *__restrict__ w = MASTER ? further<GI2D_F32>(t.w, base) : p;
+    float *__restrict__ sm = t.sm + block, *__restrict__ sv = t.sv + block;
+    Four<GT> gq[BLOCKS8];
+    Four<WT> wq[BLOCKS8];
+    unsigned mc[BLOCKS8], vc[BLOCKS8];
+    float km[BLOCKS8], kv[BLOCKS8];
     const bool groups = t.vec && n >= 4;  // (see adamw_step_kernel)
     if (groups) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const long long i = i0 + u * GI2D_ADAMW_BLOCK;
+        for (int u = 0; u < BLOCKS8; ++u) {
+            const unsigned i = 4 * lane + u * GI2D_ADAMW_BLOCK;
             const bool whole = i + 4 <= n;
             gq[u].template load<NT>(g, i, whole);
-            wq[u].template load<NT>(w_in, i, whole);
-            mc[u] = load_vec<NT>((const unsigned *)(m + (whole ? i : 0)));
-            vc[u] = load_vec<NT>((const unsigned *)(v + (whole ? i : 0)));
+            wq[u].template load<NT>(w, i, whole);
+            mc[u] = load_vec<NT>(at((const unsigned *)m, whole ? i : 0u));
+            vc[u] = load_vec<NT>(at((const unsigned *)v, whole ? i : 0u));
         }
     }
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        km[u] = sm[block + (second ? u : 0)];
-        kv[u] = sv[block + (second ? u : 0)];
-        const long long i = i0 + u * GI2D_ADAMW_BLOCK;
+    for (int u = 0; u < BLOCKS8; ++u) {
+        km[u] = sm[u < blocks ? u : 0];
+        kv[u] = sv[u < blocks ? u : 0];
+        const unsigned i = 4 * lane + u * GI2D_ADAMW_BLOCK;
         if (i < n && (!groups || i + 4 > n)) {
             gq[u].load_each(g, i, n);
-            wq[u].load_each(w_in, i, n);
+            wq[u].load_each(w, i, n);
             mc[u] = load_codes(m, i, n);
             vc[u] = load_codes(v, i, n);
         }
     }
+    int em = 0, er = 0;  // lane u: the exponents of block u
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        if (u == 1 && !second) return;
-        const long long i = i0 + u * GI2D_ADAMW_BLOCK;
+    for (int u = 0; u < BLOCKS8; ++u) {
+        if (u >= blocks) break;
+        const unsigned i = 4 * lane + u * GI2D_ADAMW_BLOCK;
         float gx[4], wx[4];
         gq[u].get(gx);
         wq[u].get(wx);
-        if ((block + u + 1) * GI2D_ADAMW_BLOCK > n) {
+        if ((unsigned)(u + 1) * GI2D_ADAMW_BLOCK > n) {
             // outside the tensor: zeros, which are no block's largest
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -544,22 +596,24 @@ __global__ __launch_bounds__(ADAMW_THREADS) void adamw_step8_kernel(
                     vc[u] &= ~(255u << (8 * j));
                 }
         }
-        const Codes8 c = step8(h, gx, clip, wx, mc[u], vc[u], km[u], kv[u], number + u);
+        const Codes8 c = step8(f, h.key, gx, wx, mc[u], vc[u], km[u], kv[u], number + u);
         if (groups && i + 4 <= n) {
             store4<PT, NT>(p, i, wx);
             if (MASTER) store4<GI2D_F32, NT>(w, i, wx);
-            store_vec<NT>((unsigned *)(m + i), c.m);
-            store_vec<NT>((unsigned *)(v + i), c.r);
+            store_vec<NT>(at((unsigned *)m, i), c.m);
+            store_vec<NT>(at((unsigned *)v, i), c.r);
         } else if (i < n) {
             store_each<PT>(p, i, n, wx);
             if (MASTER) store_each<GI2D_F32>(w, i, n, wx);
             store_codes(m, i, n, c.m);
             store_codes(v, i, n, c.r);
         }
-        if (lane == 0) {
-            sm[block + u] = exponent_scale(c.km);
-            sv[block + u] = exponent_scale(c.kr);
-        }
+        em = lane == u ? c.km : em;
+        er = lane == u ? c.kr : er;
+    }
+    if (lane < blocks) {
+        sm[lane] = __uint_as_float((unsigned)(em + 127) << 23);
+        sv[lane] = __uint_as_float((unsigned)(er + 127) << 23);
     }
 }
 
@@ -805,7 +859,8 @@ static int adamw_run(int num_tensors, const gi2d_adamw_tensor *ts, bool stream_p
         block0 += (unsigned)((t.numel + GI2D_ADAMW_BLOCK - 1) / GI2D_ADAMW_BLOCK);
         if (t.numel == 0 || t.param_type != PT || t.grad_type != GT || (t.master != nullptr) != MASTER)
             continue;
-        const int more = (int)((t.numel + ADAMW_CHUNK - 1) / ADAMW_CHUNK);
+        constexpr int chunk = BITS == 8 ? ADAMW_CHUNK8 : ADAMW_CHUNK;
+        const int more = (int)((t.numel + chunk - 1) / chunk);
         if (count == N || chunks + more > ADAMW_MAX_CHUNKS) {
             const int rc = flush();
             if (rc != GI2D_OK) return rc;
