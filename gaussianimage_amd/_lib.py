@@ -149,7 +149,7 @@ SIGNATURES = {
     "gi2d_adamw_step": (_i, [_i, ctypes.POINTER(AdamWTensor), ctypes.POINTER(AdamWHyper), _vp,
                              _vp]),
     "gi2d_grad_norm_workspace": (_i64, [_i]),
-    "gi2d_grad_norm": (_i, [_i, _vp, _vp, _vp, ctypes.c_double, _vp, _vp, _vp]),
+    "gi2d_grad_norm": (_i, [_i, _vp, _vp, _vp, ctypes.c_double, _vp, _vp, _vp, _vp]),
     "gi2d_rasterize_sum_bwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _convp, _vp, _vp,
                                     _vp, _vp, _vp, _vp]),
 }

@@ -253,7 +253,7 @@ class _ctypes_binding:
             check(lib.gi2d_grad_norm(n, (ctypes.c_void_p * n)(*[ops._ptr(g) for g in grads]),
                                      (ctypes.c_int64 * n)(*[g.numel() for g in grads]),
                                      (ctypes.c_int * n)(*[_TYPES[g.dtype] for g in grads]),
-                                     max_norm, work.data_ptr(), out.data_ptr(),
+                                     max_norm, work.data_ptr(), None, out.data_ptr(),
                                      ops._stream(device)), "gi2d_grad_norm")
         return out[0], out[1]
 

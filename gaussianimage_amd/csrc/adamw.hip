@@ -663,10 +663,15 @@ __global__ void adamw_scalars_kernel(AdamWScalars h, double beta1, double beta2,
 // ---- norm of all gradients ---------------------------------------------------------------------
 // Each workgroup sums the squares of its chunks in double (no overflow, and the sum of 2^28 squares
 // is as exact as one of them) and leaves one partial; one workgroup adds the partials in a fixed
-// order: the same bits in every run, no atomics, no memory to clear.
+// order: the same bits in every run.
 #define NORM_THREADS 256
 #define NORM_TENSORS 232
-#define NORM_GROUPS 2048
+#ifndef NORM_GROUPS
+#define NORM_GROUPS 1024
+#endif
+#ifndef NORM_ARRIVALS
+#define NORM_ARRIVALS 256
+#endif
 #ifndef NORM_SMALL_BYTES
 #define NORM_SMALL_BYTES ((int64_t)32 << 20)
 #endif
@@ -681,7 +686,7 @@ struct NormEntry {
 struct NormTable {
     int first[NORM_TENSORS];  // first chunk (INT_MAX behind the last tensor)
     NormEntry e[NORM_TENSORS];
-    int chunks;
+    int chunks, groups;  // groups: workgroups of the launch
 };
 
 __device__ __forceinline__ void add_square(double &s, float x)
@@ -733,6 +738,7 @@ __device__ __forceinline__ double block_sum(double v, double *lds)
 {
 #pragma unroll
     for (int d = 1; d < WAVE; d <<= 1) v = v + __shfl_xor(v, d);
+    __syncthreads();  // (the previous sum has been read)
     if ((threadIdx.x & (WAVE - 1)) == 0) lds[threadIdx.x / WAVE] = v;
     __syncthreads();
     double t = 0.0;
@@ -741,46 +747,20 @@ __device__ __forceinline__ double block_sum(double v, double *lds)
     return t;
 }
 
-template <int LOADS>
-__global__ __launch_bounds__(NORM_THREADS) void grad_squares_kernel(NormTable T, double *partials)
+// Sums the partials in a fixed order and writes out[0] = norm, out[1] = min(1, max_norm / (norm +
+// 1e-6)); one workgroup.  The root in float of a sum brought to [1/2, 2) by an even power of two:
+// sums beyond fp32's range have norms within it.
+__device__ __forceinline__ void finish_norm(const double *partials, int n, float max_norm, float *out,
+                                            double *lds)
 {
-    __shared__ double lds[NORM_THREADS / WAVE];
-    const int lane = threadIdx.x & (WAVE - 1);
-    static_assert(NORM_TENSORS > 3 * WAVE && NORM_TENSORS <= 4 * WAVE, "four ballots");
-    const int f0 = T.first[lane], f1 = T.first[lane + WAVE], f2 = T.first[lane + 2 * WAVE];
-    const bool in3 = lane + 3 * WAVE < NORM_TENSORS;
-    const int f3 = T.first[in3 ? lane + 3 * WAVE : NORM_TENSORS - 1];
-    double s[4] = {0.0, 0.0, 0.0, 0.0};
-    for (int c = (int)blockIdx.x; c < T.chunks; c += (int)gridDim.x) {
-        const int k = __popcll(__ballot(f0 <= c)) + __popcll(__ballot(f1 <= c)) +
-                      __popcll(__ballot(f2 <= c)) + __popcll(__ballot(f3 <= c && in3)) - 1;
-        const NormEntry e = T.e[k];
-        const void *g = pointer48<const void>(e.g, e.more);
-        const long long chunk = c - T.first[k], n = ((long long)(e.more >> 24 & 15) << 32) | e.numel;
-        const bool vec = !(e.more & 0x40000u);
-        switch (e.more >> 16 & 3) {
-            case GI2D_F32: chunk_squares<GI2D_F32, LOADS>(g, n, chunk, vec, s); break;
-            case GI2D_BF16: chunk_squares<GI2D_BF16, LOADS>(g, n, chunk, vec, s); break;
-            default: chunk_squares<GI2D_F16, LOADS>(g, n, chunk, vec, s); break;
-        }
-    }
-    const double t = block_sum((s[0] + s[1]) + (s[2] + s[3]), lds);
-    if (threadIdx.x == 0) partials[blockIdx.x] = t;
-}
-
-// out[0] = norm, out[1] = min(1, max_norm / (norm + 1e-6)).  The root in float of a sum brought
-// to [1/2, 2) by an even power of two: sums beyond fp32's range have norms within it.
-__global__ __launch_bounds__(NORM_THREADS) void grad_norm_kernel(const double *__restrict__ partials,
-                                                                 int n, float max_norm, float *out)
-{
-    __shared__ double lds[NORM_THREADS / WAVE];
     double s = 0.0;
     for (int r = 0; r < n; r += 8 * NORM_THREADS) {
         double y[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int i = r + j * NORM_THREADS + (int)threadIdx.x;
-            y[j] = partials[i < n ? i : n - 1];
+            y[j] = __hip_atomic_load(partials + (i < n ? i : n - 1), __ATOMIC_RELAXED,
+                                     __HIP_MEMORY_SCOPE_AGENT);
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) s = s + (r + j * NORM_THREADS + (int)threadIdx.x < n ? y[j] : 0.0);
@@ -800,6 +780,61 @@ __global__ __launch_bounds__(NORM_THREADS) void grad_norm_kernel(const double *_
     out[0] = norm;
     const float c = max_norm / (norm + 1e-6f);
     out[1] = c < 1.0f || c != c ? c : 1.0f;
+}
+
+// `arrived`: nullptr, or the number of workgroups that have left their partial, 0 between calls: the
+// last one to arrive finishes the norm (`before`: partials of earlier launches of this call).  The
+// order of arrival chooses who adds the partials, not the order in which they are added.
+template <int LOADS>
+__global__ __launch_bounds__(NORM_THREADS) void grad_squares_kernel(NormTable T, double *partials,
+                                                                    int before, unsigned *arrived,
+                                                                    float max_norm, float *out)
+{
+    __shared__ double lds[NORM_THREADS / WAVE];
+    __shared__ unsigned place;
+    const int lane = threadIdx.x & (WAVE - 1);
+    static_assert(NORM_TENSORS > 3 * WAVE && NORM_TENSORS <= 4 * WAVE, "four ballots");
+    const int f0 = T.first[lane], f1 = T.first[lane + WAVE], f2 = T.first[lane + 2 * WAVE];
+    const bool in3 = lane + 3 * WAVE < NORM_TENSORS;
+    const int f3 = T.first[in3 ? lane + 3 * WAVE : NORM_TENSORS - 1];
+    double s[4] = {0.0, 0.0, 0.0, 0.0};
+    for (int c = (int)blockIdx.x; c < T.chunks; c += T.groups) {
+        const int k = __popcll(__ballot(f0 <= c)) + __popcll(__ballot(f1 <= c)) +
+                      __popcll(__ballot(f2 <= c)) + __popcll(__ballot(f3 <= c && in3)) - 1;
+        const NormEntry e = T.e[k];
+        const void *g = pointer48<const void>(e.g, e.more);
+        const long long chunk = c - T.first[k], n = ((long long)(e.more >> 24 & 15) << 32) | e.numel;
+        const bool vec = !(e.more & 0x40000u);
+        switch (e.more >> 16 & 3) {
+            case GI2D_F32: chunk_squares<GI2D_F32, LOADS>(g, n, chunk, vec, s); break;
+            case GI2D_BF16: chunk_squares<GI2D_BF16, LOADS>(g, n, chunk, vec, s); break;
+            default: chunk_squares<GI2D_F16, LOADS>(g, n, chunk, vec, s); break;
+        }
+    }
+    const double t = block_sum((s[0] + s[1]) + (s[2] + s[3]), lds);
+    if (threadIdx.x == 0) {
+        __hip_atomic_store(partials + before + blockIdx.x, t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (arrived) {
+            // The partials alone pass between workgroups, and they do not go through the L2 caches
+            // (stores and loads of agent scope): once the store has been acknowledged, whoever
+            // reads a later count finds it.  A release would write back the whole L2 of the XCD.
+            __builtin_amdgcn_s_waitcnt(0);
+            place = __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+    }
+    if (!arrived) return;
+    __syncthreads();
+    if (place != (unsigned)T.groups - 1u) return;
+    finish_norm(partials, before + T.groups, max_norm, out, lds);
+    if (threadIdx.x == 0) __hip_atomic_store(arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// The second launch of a call without `arrived`.
+__global__ __launch_bounds__(NORM_THREADS) void grad_norm_kernel(const double *partials, int n,
+                                                                 float max_norm, float *out)
+{
+    __shared__ double lds[NORM_THREADS / WAVE];
+    finish_norm(partials, n, max_norm, out, lds);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -988,7 +1023,8 @@ int64_t gi2d_grad_norm_workspace(int num_tensors)
 }
 
 int gi2d_grad_norm(int num_tensors, const void *const *grads, const int64_t *numel,
-                   const int *types, double max_norm, void *workspace, float *out, void *stream)
+                   const int *types, double max_norm, void *workspace, uint32_t *arrived, float *out,
+                   void *stream)
 {
     if (num_tensors < 0 || !out || !workspace || !(max_norm >= 0.0)) return GI2D_E_INVALID;
     if (num_tensors > 0 && (!grads || !numel || !types)) return GI2D_E_INVALID;
@@ -1006,15 +1042,20 @@ int gi2d_grad_norm(int num_tensors, const void *const *grads, const int64_t *num
     NormTable T;
     int count = 0, done = 0;
     T.chunks = 0;
-    const auto flush = [&]() {
+    const float limit = (float)max_norm;
+    bool finished = false;
+    const auto flush = [&](bool last) {
         if (count == 0) return GI2D_OK;
         for (int c = count; c < NORM_TENSORS; ++c) T.first[c] = INT_MAX;
-        const int groups = T.chunks < NORM_GROUPS ? T.chunks : NORM_GROUPS;
+        T.groups = T.chunks < NORM_GROUPS ? T.chunks : NORM_GROUPS;
+        const dim3 grid((unsigned)T.groups);
+        uint32_t *const count_in = last && T.groups <= NORM_ARRIVALS ? arrived : nullptr;
+        finished = count_in != nullptr;
         if (small)
-            grad_squares_kernel<2><<<dim3((unsigned)groups), NORM_THREADS, 0, st>>>(T, partials + done);
+            grad_squares_kernel<2><<<grid, NORM_THREADS, 0, st>>>(T, partials, done, count_in, limit, out);
         else
-            grad_squares_kernel<8><<<dim3((unsigned)groups), NORM_THREADS, 0, st>>>(T, partials + done);
-        done += groups;
+            grad_squares_kernel<8><<<grid, NORM_THREADS, 0, st>>>(T, partials, done, count_in, limit, out);
+        done += T.groups;
         count = T.chunks = 0;
         return launch_status();
     };
@@ -1023,7 +1064,7 @@ int gi2d_grad_norm(int num_tensors, const void *const *grads, const int64_t *num
         const int64_t chunk = chunk_bytes / type_size(types[i]);
         const int64_t more = (numel[i] + chunk - 1) / chunk;  // at most 2^21: 232 tensors below 2^31
         if (count == NORM_TENSORS) {
-            const int rc = flush();
+            const int rc = flush(false);
             if (rc != GI2D_OK) return rc;
         }
         T.first[count] = T.chunks;
@@ -1034,9 +1075,9 @@ int gi2d_grad_norm(int num_tensors, const void *const *grads, const int64_t *num
         T.chunks += (int)more;
         ++count;
     }
-    int rc = flush();
-    if (rc != GI2D_OK) return rc;
-    grad_norm_kernel<<<1, NORM_THREADS, 0, st>>>(partials, done, (float)max_norm, out);
+    const int rc = flush(true);
+    if (rc != GI2D_OK || finished) return rc;
+    grad_norm_kernel<<<1, NORM_THREADS, 0, st>>>(partials, done, limit, out);
     return launch_status();
 }
 

@@ -247,6 +247,25 @@ void step(const char *op, int bits, const py::object &params_, const py::object 
     for (c10::TensorImpl *t : out) written(t);
 }
 
+// The word of a stream that gi2d_grad_norm's workgroups count their arrivals in (0 between calls;
+// kept for the life of the process).  nullptr while the stream is captured: a graph may be replayed
+// next to another one that was captured on the same stream.
+uint32_t *arrivals(const at::Device &device, hipStream_t stream)
+{
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(stream, &capture) != hipSuccess) {
+        (void)hipGetLastError();
+        return nullptr;
+    }
+    if (capture != hipStreamCaptureStatusNone) return nullptr;
+    static std::mutex lock;
+    static auto &words = *new std::map<std::pair<int, hipStream_t>, at::Tensor>();
+    std::lock_guard<std::mutex> hold(lock);
+    at::Tensor &t = words[{(int)device.index(), stream}];
+    if (!t.defined()) t = at::zeros({1}, at::TensorOptions().dtype(at::kInt).device(device));
+    return reinterpret_cast<uint32_t *>(t.data_ptr<int>());
+}
+
 py::tuple grad_norm(const py::object &grads_, double max_norm)
 {
     static const char *const op = "grad_norm";
@@ -276,8 +295,9 @@ py::tuple grad_norm(const py::object &grads_, double max_norm)
         c10::GetAllocator(device.type())->allocate((size_t)gi2d_grad_norm_workspace((int)n));
     const at::AutoDispatchBelowADInplaceOrView no_autograd;
     const at::Tensor out = at::empty({2}, at::TensorOptions().dtype(at::kFloat).device(device));
+    const hipStream_t stream = c10::hip::getCurrentHIPStream(device.index()).stream();
     check(gi2d_grad_norm((int)n, ptr.data(), numel.data(), type.data(), max_norm, work.get(),
-                         out.data_ptr<float>(), c10::hip::getCurrentHIPStream(device.index()).stream()),
+                         arrivals(device, stream), out.data_ptr<float>(), stream),
           "gi2d_grad_norm", true);
     return py::make_tuple(out.select(0, 0), out.select(0, 1));
 }

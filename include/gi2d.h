@@ -354,10 +354,13 @@ int gi2d_adamw_step(int num_tensors, const gi2d_adamw_tensor *tensors,
 /* 2-norm of all gradients together: out[0] = sqrt(sum g^2), summed in double and in a fixed order,
  * out[1] = min(1, max_norm / (out[0] + 1e-6)).  Host arrays of device pointers, element counts and
  * element types; `workspace`: gi2d_grad_norm_workspace(num_tensors) bytes of device memory that
- * belong to this call until it has run; out: two floats in device memory. */
+ * belong to this call until it has run; arrived: NULL, or one word of device memory that is 0 before
+ * the call and 0 again when it has run, and that no call uses meanwhile (with it the norm is
+ * finished by the last workgroup instead of a second launch); out: two floats in device memory. */
 int64_t gi2d_grad_norm_workspace(int num_tensors);
 int gi2d_grad_norm(int num_tensors, const void *const *grads, const int64_t *numel,
-                   const int *types, double max_norm, void *workspace, float *out, void *stream);
+                   const int *types, double max_norm, void *workspace, uint32_t *arrived, float *out,
+                   void *stream);
 
 /* Fused fitting iteration on the model's RAW parameters -- the caller's loop of
  * gaussianimage_cholesky.py:101-124 / gaussianimage_rs.py:82-95 (forward, L2

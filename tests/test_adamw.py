@@ -211,7 +211,7 @@ def test_c_entries_refuse_without_a_device():
               (1, (ctypes.c_void_p * 1)(None), size, kind, 1.0, 64, 64),
               (1, one, (ctypes.c_int64 * 1)(-1), kind, 1.0, 64, 64),
               (1, one, size, (ctypes.c_int * 1)(3), 1.0, 64, 64)):
-        assert lib.gi2d_grad_norm(*a, None) == bad, a
+        assert lib.gi2d_grad_norm(*a[:6], None, *a[6:], None) == bad, a
 
 
 # ------------------------------------------------------------------ GPU: helpers
