@@ -185,11 +185,6 @@ class _ctypes_binding:
                     refuse("masters", "must be a float32 tensor laid out as its parameter")
                 t.master = ops._ptr(w)
                 out.append(w)
-            if t.numel:
-                for x in out:
-                    if x.data_ptr() in seen:
-                        refuse("params", "or its state appears twice")
-                    seen.add(x.data_ptr())
             if bits == 8:
                 blocks = (t.numel + ADAMW_BLOCK - 1) // ADAMW_BLOCK
                 for name, x in list(names.items())[4:6]:
@@ -198,6 +193,12 @@ class _ctypes_binding:
                         refuse(name, "must be a contiguous float32 tensor with one element for 256 "
                                "of the parameter's, on its device")
                 t.exp_avg_scale, t.exp_avg_sq_scale = ops._ptr(scales[i]), ops._ptr(sq_scales[i])
+                out += [scales[i], sq_scales[i]]
+            if t.numel:
+                for x in out:
+                    if x.data_ptr() in seen:
+                        refuse("params", "or its state appears twice")
+                    seen.add(x.data_ptr())
         ops._need_cuda(op, params[0])
         h = _lib.AdamWHyper(beta1=betas[0], beta2=betas[1], eps=eps, weight_decay=weight_decay, seed=seed,
                             state_bits=bits, step=1)

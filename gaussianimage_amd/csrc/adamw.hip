@@ -13,10 +13,14 @@
 #include "host.h"
 
 #define ADAMW_THREADS 256
-#define ADAMW_CHUNK 2048          // elements of a workgroup, 8 per lane
-#ifndef BLOCKS8
-#define BLOCKS8 4                 // blocks of 256 of a wave with 8-bit states
-#endif
+// Groups of four elements of a lane with 32-bit states.  Through the caches 2: 5.8 M fp32 elements
+// took 26 us with them, 28 with 1 or 4.  Streamed 4: 150 M 711 us against 733 with 2, 333 M 1611
+// against 1642 (100 M the same; with 1 they vary with where the arrays lie, 5.3 to 6.0 TB/s).
+#define GROUPS32(NT) ((NT) ? 4 : 2)
+#define ADAMW_CHUNK32(NT) (GROUPS32(NT) * 4 * ADAMW_THREADS)  // elements of a workgroup
+// Blocks of 256 elements of a wave with 8-bit states: 120 M fp32 elements 311 us, 109 M bf16 177;
+// with 2 blocks 314 and 188.
+#define BLOCKS8 4
 #define ADAMW_CHUNK8 (ADAMW_THREADS / WAVE * BLOCKS8 * GI2D_ADAMW_BLOCK)
 #define ADAMW_MAX_NUMEL ((int64_t)1 << 34)
 #define ADAMW_MAX_CHUNKS (1 << 23)  // chunks of a launch: 256 lanes each, below 2^32 lanes
@@ -79,6 +83,7 @@ struct AdamWTable {
     // 27: the upper bits of numel; 31: every pointer allows four elements per access
     unsigned meta[N];
     Entry e[N];
+    static_assert(sizeof(Entry) % 4 == 0 && alignof(Entry) == 4, "words only");
 };
 #define META_FIRST 0xffffffu
 #define META_VEC 0x80000000u
@@ -247,17 +252,18 @@ __global__ __launch_bounds__(ADAMW_THREADS) void adamw_step_kernel(
     const auto t = tensor_of(T);
     const AdamWScalars h = scalars_of(ha, h_dev);
     const float clip = clip_dev ? *clip_dev : 1.0f;
-    const long long base = (long long)t.chunk * ADAMW_CHUNK;
-    const unsigned n = t.n - base < ADAMW_CHUNK ? (unsigned)(t.n - base) : ADAMW_CHUNK;  // of this chunk
+    constexpr int GROUPS = GROUPS32(NT), CHUNK = ADAMW_CHUNK32(NT);
+    const long long base = (long long)t.chunk * CHUNK;
+    const unsigned n = t.n - base < CHUNK ? (unsigned)(t.n - base) : CHUNK;  // of this chunk
     constexpr int WT = MASTER ? GI2D_F32 : PT;  // what is read and updated
     void *__restrict__ p = further<PT>(t.p, base);
     const void *__restrict__ g = further<GT>(t.g, base);
     void *__restrict__ m = further<GI2D_F32>(t.m, base);
     void *__restrict__ v = further<GI2D_F32>(t.v, base);
     void *__restrict__ w = MASTER ? further<GI2D_F32>(t.w, base) : p;
-    Four<GT> gq[2];
-    Four<WT> wq[2];
-    Four<GI2D_F32> mq[2], vq[2];
+    Four<GT> gq[GROUPS];
+    Four<WT> wq[GROUPS];
+    Four<GI2D_F32> mq[GROUPS], vq[GROUPS];
     const unsigned i0 = 4 * threadIdx.x;
     // Groups that lie inside load at once, those outside load anything; the one across the end of
     // the tensor -- or every one of a tensor that allows single elements only -- then loads again,
@@ -266,8 +272,8 @@ __global__ __launch_bounds__(ADAMW_THREADS) void adamw_step_kernel(
     const bool groups = t.vec && n >= 4;
     if (groups) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const unsigned i = i0 + u * (ADAMW_CHUNK / 2);
+        for (int u = 0; u < GROUPS; ++u) {
+            const unsigned i = i0 + u * (4 * ADAMW_THREADS);
             const bool whole = i + 4 <= n;
             gq[u].template load<NT>(g, i, whole);
             wq[u].template load<NT>(w, i, whole);
@@ -276,8 +282,8 @@ __global__ __launch_bounds__(ADAMW_THREADS) void adamw_step_kernel(
         }
     }
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const unsigned i = i0 + u * (ADAMW_CHUNK / 2);
+    for (int u = 0; u < GROUPS; ++u) {
+        const unsigned i = i0 + u * (4 * ADAMW_THREADS);
         if (i < n && (!groups || i + 4 > n)) {
             gq[u].load_each(g, i, n);
             wq[u].load_each(w, i, n);
@@ -286,8 +292,8 @@ __global__ __launch_bounds__(ADAMW_THREADS) void adamw_step_kernel(
         }
     }
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const unsigned i = i0 + u * (ADAMW_CHUNK / 2);
+    for (int u = 0; u < GROUPS; ++u) {
+        const unsigned i = i0 + u * (4 * ADAMW_THREADS);
         float gx[4], wx[4], mx[4], vx[4];
         gq[u].get(gx);
         wq[u].get(wx);
@@ -416,29 +422,40 @@ struct Codes8 {
     int km, kr;        // the block's exponents
 };
 
-// The factors of step8, the clip coefficient and the roots of those of the square folded in, and
-// the step size into the denominator.  (A step size of 0 makes the denominator's factors the
-// largest number: the quotient is 0.)
+// The factors of step8: the step size is folded into those of the denominator.  (A step size of 0
+// makes them the largest number: the quotient is 0.)
 struct Factors8 {
-    float b1, g_m, root_b2, g_r, decay, d_r, d_eps;
-    __device__ __forceinline__ Factors8(const AdamWScalars &h, float clip)
+    float b1, omb1, b2, omb2, clip, decay, d_r, d_eps;
+    __device__ __forceinline__ Factors8(const AdamWScalars &h, float c)
     {
         const float most = 3.402823466e38f;
         b1 = H_B1(h);
-        g_m = H_OMB1(h) * clip;
-        root_b2 = sqrtf(H_B2(h));
-        g_r = sqrtf(H_OMB2(h)) * clip;
+        omb1 = H_OMB1(h);
+        b2 = H_B2(h);
+        omb2 = H_OMB2(h);
+        clip = c;
         decay = H_DECAY(h);
         d_r = fminf(H_INV_BC2(h) / H_STEP(h), most);
         d_eps = fminf(H_EPS(h) / H_STEP(h), most);
     }
 };
 
+// Square root of a normal number: the reciprocal root's approximation times x, and one step of
+// Newton's with the exact residual.  Correctly rounded but for one in some millions of numbers (and
+// next to the smallest normal ones); sqrtf's 14 instructions settle those as well.
+__device__ __forceinline__ float root_normal(float x)
+{
+    const float y = __builtin_amdgcn_rsqf(x);
+    const float s = x * y;
+    return __builtin_fmaf(__builtin_fmaf(-s, s, x), 0.5f * y, s);
+}
+
 // Four neighbouring elements of a lane, the wave holding their block: the update of p, and the new
-// codes.  The root and the reciprocal are the hardware's, one unit in the last place each, and sums
-// of products are fused: a ten-millionth of the step.  (Correctly rounded root and quotient took
-// half the instructions of the kernel: 10 bytes per element leave 266 cycles for 64 of them, and an
-// instruction takes 4, before the instructions and not the memory set the time.)
+// codes.  What the codes are made of is rounded operation by operation, as the formulas are written
+// down: a last bit would send one value in a million to another code, 6 to 12 % away.  The step of
+// p takes the hardware's reciprocal (one unit in the last place) and fused sums, a ten-millionth of
+// the step: 10 bytes per element leave 266 cycles for 64 of them, and an instruction takes 4, before
+// the instructions and not the memory set the time.
 __device__ __forceinline__ Codes8 step8(const Factors8 &f, unsigned key, const float *g, float *p,
                                         unsigned cm, unsigned cr, float sm, float sr, unsigned block)
 {
@@ -446,25 +463,37 @@ __device__ __forceinline__ Codes8 step8(const Factors8 &f, unsigned key, const f
     float m[4], r[4];
     decode4(cm, m);
     decode4(cr, r);
-    const float m_b1 = sm * f.b1, r_b2 = sr * f.root_b2;  // (powers of two times the factors)
-    unsigned long long tiny = 0;
+    // The scales are powers of two: they change no rounding, wherever in a product they stand, as
+    // long as their square is a normal number.
+    const float m_b1 = sm * f.b1;
+    const bool plain = sr >= 0x1p-50f && sr <= 0x1p50f;
+    const float v_b2 = plain ? sr * sr * f.b2 : f.b2;
+    if (!plain) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[j] = r[j] * sr;
+    }
+    unsigned long long odd = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        m[j] = __builtin_fmaf(m[j], m_b1, g[j] * f.g_m);
-        const float old = r[j] * r_b2, now = g[j] * f.g_r;
-        r[j] = __builtin_fmaf(old, old, now * now);
-        tiny |= __builtin_amdgcn_ballot_w64(__builtin_amdgcn_classf(r[j], 0x80));  // a positive subnormal
+        const float gj = g[j] * f.clip;
+        m[j] = m[j] * m_b1 + gj * f.omb1;
+        r[j] = (r[j] * r[j]) * v_b2 + (gj * gj) * f.omb2;
+        // zero, a positive subnormal, infinity
+        odd |= __builtin_amdgcn_ballot_w64(__builtin_amdgcn_classf(r[j], 0x2c0));
     }
-    if (tiny != 0) {  // (the instruction takes subnormals for zeros)
+    unsigned least[4];  // of the root's code, in bits 24 to 30
+    if (odd != 0) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const bool small = r[j] < 0x1p-64f;
-            const float root = __builtin_amdgcn_sqrtf(small ? r[j] * 0x1p64f : r[j]);
-            r[j] = small ? root * 0x1p-32f : root;
+            r[j] = sqrtf(r[j]);
+            least[j] = r[j] > 0.0f ? 0x1000000u : 0u;
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) r[j] = __builtin_amdgcn_sqrtf(r[j]);
+        for (int j = 0; j < 4; ++j) {
+            r[j] = root_normal(r[j]);
+            least[j] = 0x1000000u;
+        }
     }
     unsigned ar[4];  // a root has no sign (a NaN may: it is above everything)
 #pragma unroll
@@ -511,11 +540,11 @@ __device__ __forceinline__ Codes8 step8(const Factors8 &f, unsigned key, const f
         }
     }
     // A root that is not zero stays so: with a mean beside it, the next step would divide by eps
-    // alone.  (The root of an fp32 number is 0 or above 2^-76: its bits are above 1 << 24.)
+    // alone.
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         em[j] = (em[j] & 0x7fffffffu) | (__float_as_uint(m[j]) & 0x80000000u);
-        er[j] = up(er[j], ar[j] < 0x1000000u ? ar[j] : 0x1000000u);
+        er[j] = up(er[j], least[j]);
     }
     out.m = pack_upper(em);
     out.r = pack_upper(er);
@@ -748,8 +777,8 @@ __device__ __forceinline__ double block_sum(double v, double *lds)
 }
 
 // Sums the partials in a fixed order and writes out[0] = norm, out[1] = min(1, max_norm / (norm +
-// 1e-6)); one workgroup.  The root in float of a sum brought to [1/2, 2) by an even power of two:
-// sums beyond fp32's range have norms within it.
+// 1e-6)); one workgroup.  The root of the sum brought to [1/2, 2) by an even power of two: sums
+// beyond fp32's range have norms within it.
 __device__ __forceinline__ void finish_norm(const double *partials, int n, float max_norm, float *out,
                                             double *lds)
 {
@@ -775,7 +804,9 @@ __device__ __forceinline__ void finish_norm(const double *partials, int n, float
             f = f * 2.0;
             e -= 1;
         }
-        norm = ldexpf(sqrtf((float)f), e / 2);
+        // (one step of Newton's from the float root r; f - r^2 is exact)
+        const float r = sqrtf((float)f);
+        norm = ldexpf((float)((double)r + (f - (double)r * (double)r) * (double)(0.5f / r)), e / 2);
     }
     out[0] = norm;
     const float c = max_norm / (norm + 1e-6f);
@@ -894,7 +925,7 @@ static int adamw_run(int num_tensors, const gi2d_adamw_tensor *ts, bool stream_p
         block0 += (unsigned)((t.numel + GI2D_ADAMW_BLOCK - 1) / GI2D_ADAMW_BLOCK);
         if (t.numel == 0 || t.param_type != PT || t.grad_type != GT || (t.master != nullptr) != MASTER)
             continue;
-        constexpr int chunk = BITS == 8 ? ADAMW_CHUNK8 : ADAMW_CHUNK;
+        const int chunk = BITS == 8 ? ADAMW_CHUNK8 : ADAMW_CHUNK32(stream_past);
         const int more = (int)((t.numel + chunk - 1) / chunk);
         if (count == N || chunks + more > ADAMW_MAX_CHUNKS) {
             const int rc = flush();

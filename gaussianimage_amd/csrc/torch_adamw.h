@@ -65,25 +65,38 @@ inline bool same_layout(const at::Tensor &t, const at::Tensor &p, bool p_contigu
 }
 
 // Set of addresses that a call writes: a tensor given twice would be updated by two workgroups at
-// once.
+// once.  (One table for each thread, emptied by counting calls.)
 class Written {
-    std::vector<const void *> slots;
+    struct Slot {
+        const void *p = nullptr;
+        uint64_t call = 0;
+    };
+    static std::vector<Slot> &table()
+    {
+        static thread_local std::vector<Slot> slots;
+        return slots;
+    }
+    std::vector<Slot> &slots;
     size_t mask;
+    uint64_t call;
 
   public:
-    explicit Written(size_t n)
+    explicit Written(size_t n) : slots(table())
     {
-        size_t size = 16;
+        static thread_local uint64_t calls = 0;
+        size_t size = 64;
         while (size < 2 * n) size *= 2;
-        slots.assign(size, nullptr);
-        mask = size - 1;
+        if (slots.size() < size) slots.assign(size, Slot());
+        mask = slots.size() - 1;
+        call = ++calls;
     }
     bool add(const void *p)
     {
         size_t at = ((uintptr_t)p >> 4) * 0x9E3779B97F4A7C15ull >> 32 & mask;
-        for (; slots[at] != nullptr; at = (at + 1) & mask)
-            if (slots[at] == p) return false;
-        slots[at] = p;
+        for (; slots[at].call == call; at = (at + 1) & mask)
+            if (slots[at].p == p) return false;
+        slots[at].p = p;
+        slots[at].call = call;
         return true;
     }
 };
@@ -160,10 +173,11 @@ void step(const char *op, int bits, const py::object &params_, const py::object 
     const char *state_what = bits == 8 ? "must be a float8_e4m3fn tensor laid out as its parameter"
                                        : "must be a float32 tensor laid out as its parameter";
     const at::Device device = params.at(0)->device();
-    std::vector<gi2d_adamw_tensor> ts((size_t)n);
-    std::vector<c10::TensorImpl *> out;  // what the call writes
-    out.reserve((size_t)n * 6);
-    Written seen((size_t)n * 4);
+    static thread_local std::vector<gi2d_adamw_tensor> ts;
+    static thread_local std::vector<c10::TensorImpl *> out;  // what the call writes
+    if (ts.size() < (size_t)n) ts.resize((size_t)n);
+    out.clear();
+    Written seen((size_t)n * 6);
     for (int64_t i = 0; i < n; ++i) {
         const at::Tensor &p = *params.at(i), &g = *grads.at(i), &mi = *m.at(i), &vi = *v.at(i);
         const at::Tensor *w = masters.at(i, true);
@@ -218,6 +232,8 @@ void step(const char *op, int bits, const py::object &params_, const py::object 
             if (t.numel) {
                 t.exp_avg_scale = a.data_ptr<float>();
                 t.exp_avg_sq_scale = b.data_ptr<float>();
+                if (!seen.add(t.exp_avg_scale) || !seen.add(t.exp_avg_sq_scale))
+                    refuse(op, "params", i, "or its state appears twice");
             }
         }
     }

@@ -12,13 +12,12 @@ u = 2.0 ** -24
 BLOCK = 256
 
 
-def step(p, g, m, v, t, lr, betas, eps, weight_decay, clip=1.0, more=0, bits=32):
+def step(p, g, m, v, t, lr, betas, eps, weight_decay, clip=1.0, more=0):
     """New (p, m, v) and the bounds of their float32 counterparts.  Inputs are the float32 (or
     half) values, exactly; ``clip`` the float32 coefficient, ``more`` the roundings by which it may
-    itself be off.  With 8-bit states the root and the reciprocal of the denominator are the
-    hardware's, a unit in the last place (2 roundings) each: the root 4.5 from v and 2, the
-    denominator's factors 3 each (itself, the step size, their quotient), its sum 1, the reciprocal
-    2, the difference 1: 13.5, below the 14 counted here."""
+    itself be off.  The parameter with 8-bit states: the root 3.5 from v and 1, the denominator's
+    factors 3 each (itself, the step size, their quotient), its sum 1, the hardware's reciprocal a
+    unit in the last place (2), the difference 1: 11.5, below the 14 counted here."""
     p, g, m, v = (np.asarray(x, np.float64) for x in (p, g, m, v))
     b1, b2 = betas
     g = g * clip                                     # 1 rounding of g
@@ -27,9 +26,8 @@ def step(p, g, m, v, t, lr, betas, eps, weight_decay, clip=1.0, more=0, bits=32)
     tol_m = u * (4 * np.abs(b1 * m) + (4 + more) * np.abs((1 - b1) * g)) + 2.0 ** -149
     v_new = b2 * v + (1 - b2) * g * g
     # all terms positive: g twice, g*g, coefficient, product, sum (v itself may be a rounded
-    # square: 1 more).  With 8-bit states g times the root of the coefficient is squared: the root
-    # 1.5, the clip coefficient 1, g 1, twice each, the square 1 and the sum 1
-    tol_v = ((9 if bits == 8 else 7) + 2 * more) * u * v_new + 2.0 ** -148
+    # square: 1 more)
+    tol_v = (7 + 2 * more) * u * v_new + 2.0 ** -148
     step_size = lr / (1 - b1 ** t)
     denom = np.sqrt(v_new / (1 - b2 ** t)) + eps
     with np.errstate(divide="ignore", invalid="ignore"):

@@ -151,6 +151,8 @@ def test_refused_tensors(binding):
         eight(a, sa, b, sb.double())
     with pytest.raises(ValueError, match="twice"):
         eight(a, sa, a, sb)
+    with pytest.raises(ValueError, match="twice"):
+        eight(a, sa, b, sa)
     with pytest.raises(ValueError, match="no gradients"):
         grad_norm([])
     with pytest.raises(ValueError, match="gaps"):
@@ -269,7 +271,7 @@ class Case:
         block, wrong, total = 0, 0, 0
         for i, n in enumerate(self.sizes):
             w, g, m, v = self.np[i]
-            p2, m2, v2, tp, tm, tv = O.step(w, g, m, v, t, lr, betas, eps, wd, clip, bits=self.bits)
+            p2, m2, v2, tp, tm, tv = O.step(w, g, m, v, t, lr, betas, eps, wd, clip)
             p, master = self.cols["p"][i], self.cols["w"][i]
             if master is not None:
                 _near(master, p2, tp, f"master {i}")
@@ -339,6 +341,47 @@ SIZES = [1, 2, 3, 255, 256, 257, 0, 2047, 2048, 2049, 4096, 5003]
 @pytest.mark.parametrize("pt,gt,master", TYPES, ids=IDS)
 def test_step(bits, pt, gt, master, off, binding):
     c = Case(SIZES, pt, gt, bits, master, off, seed=off + 1)
+    c.run()
+    c.check()
+
+
+def _filler(bits, pt, gt, master, nbytes):
+    """A tensor of zeros that makes a call touch more than ``nbytes``."""
+    from gaussianimage_amd.adamw import zero_state_8bit
+    n = nbytes // 8
+    p = torch.zeros(n, dtype=pt, device=DEV)
+    m = zero_state_8bit(p) if bits == 8 else (torch.zeros(n, device=DEV), None, torch.zeros(n, device=DEV), None)
+    return dict(p=p, g=torch.zeros(n, dtype=gt, device=DEV), m=m[0], sm=m[1], v=m[2], sv=m[3],
+                w=torch.zeros(n, device=DEV) if master else None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("off", [0, 1])
+@pytest.mark.parametrize("pt,gt,master", [(F32, F32, False), (BF16, BF16, True), (F16, F32, False)],
+                         ids=["f32", "bf16-master", "f16-f32"])
+def test_step_of_a_call_beyond_the_cache(bits, off, pt, gt, master):
+    """The streamed kernels, on the sizes where they can go wrong; a tensor behind the long one
+    (its blocks' numbers in the 8-bit rounding count on)."""
+    c = Case(SIZES, pt, gt, bits, master, off, seed=off + 21)
+    fill = _filler(bits, pt, gt, master, 144 << 20)
+    for k, x in c.cols.items():
+        x.append(fill[k])
+    c.run()
+    for k in ("p", "m", "v", "w"):
+        x = c.cols[k].pop()
+        assert x is None or not x.view(torch.uint8).any()
+    for k in ("g", "sm", "sv"):
+        c.cols[k].pop()
+    c.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("pt,gt,master", [(F32, F32, False), (BF16, BF16, True)], ids=["f32", "bf16-master"])
+def test_more_tensors_than_a_launch_takes(bits, pt, gt, master):
+    rng = np.random.RandomState(7)
+    c = Case([int(x) for x in rng.randint(0, 700, size=260)], pt, gt, bits, master, seed=31)
     c.run()
     c.check()
 
@@ -548,12 +591,13 @@ def test_more_than_2_31_elements(bits):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("off", [0, 1])
+@pytest.mark.parametrize("long", [0, 40 << 20], ids=["short", "long"])
 @pytest.mark.parametrize("types", [[F32], [BF16], [F16], [F32, BF16, F16]], ids=["f32", "bf16", "f16", "mixed"])
-def test_grad_norm(types, off, binding):
+def test_grad_norm(types, long, off, binding):
     from gaussianimage_amd.adamw import grad_norm
     rng = np.random.RandomState(3)
-    sizes = [1, 0, 7, 4095, 4096, 4097, 8191, 8192, 8193, 100003] + [int(rng.randint(1, 300)) for _ in range(200)]
-    grads = []
+    sizes = [1, 0, 7, 4095, 4096, 4097, 8191, 8192, 8193, 100003] + [int(rng.randint(1, 300)) for _ in range(240)]
+    grads = [torch.zeros(long // 4, device=DEV)]     # (beyond 32 MB more is loaded at once)
     for i, n in enumerate(sizes):
         buf = torch.full((n + off,), float("nan"), dtype=types[i % len(types)], device=DEV)
         buf[off:] = torch.as_tensor(rng.randn(n))
@@ -562,8 +606,7 @@ def test_grad_norm(types, off, binding):
         norm, coef = grad_norm(grads, limit)
         want, c = O.grad_norm([g.double().cpu().numpy() for g in grads], limit)
         assert norm.shape == coef.shape == () and norm.dtype == F32 and norm.device == coef.device == grads[0].device
-        # the sum in double, then one rounding to float, its root and the power of two: 2 roundings;
-        # the coefficient 3 more
+        # the sum and its root in double, one rounding to float (2 counted); the coefficient 3 more
         assert abs(float(norm) - want) <= 2 * O.u * want
         assert abs(float(coef) - c) <= 5 * O.u * c
     again, none = grad_norm(grads)
@@ -582,6 +625,28 @@ def test_grad_norm_magnitudes(size):
     else:
         assert abs(float(norm) - want) <= 2 * O.u * want + 2.0 ** -149
         assert abs(float(coef) - min(1.0, 1 / (want + 1e-6))) <= 5 * O.u
+
+
+@pytest.mark.gpu
+def test_grad_norm_on_two_streams_at_once():
+    """Each stream counts its own arrivals: short norms next to each other, many times, and a
+    long one (two launches) in between."""
+    from gaussianimage_amd.adamw import grad_norm
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    grads = [[torch.randn(n, generator=gen, device=DEV) for n in sizes] for sizes in ((200000, 77), (150001, 3, 9000))]
+    long = torch.randn(9 << 20, generator=gen, device=DEV)
+    want = [grad_norm(g, 1.0)[0].clone() for g in grads] + [grad_norm([long])[0].clone()]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for k in range(60):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got.append((i, grad_norm(grads[i], 1.0)[0]))
+                if k % 7 == i:
+                    got.append((2, grad_norm([long])[0]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[i]) for i, x in got)
 
 
 @pytest.mark.gpu
@@ -788,7 +853,7 @@ def test_optimizer_follows_the_operators(dtype, master, state_bits, binding):
                 v = v * v
             lr, wd = (1e-2, DECAY) if i < 2 else (LR, 0.1)
             new, _, _, tol, _, _ = O.step(w[i], grads[i].double().cpu().numpy(), m, v, steps[i], lr, BETAS, EPS, wd,
-                                          coef, more=6, bits=state_bits)  # the coefficient: 5, and its rounding here
+                                          coef, more=6)  # the coefficient: 5, and its rounding here
             if master:
                 _near(opt.state[p]["master"], new, tol, f"master {i}")
                 assert torch.equal(p, opt.state[p]["master"].to(dtype))
@@ -872,7 +937,7 @@ def test_an_image_fit_with_clipped_adamw(state_bits):
         _, coef = O.grad_norm(seen["grads"], 1e-3)
         for i, p in enumerate(ps):
             new, _, _, tol, _, _ = O.step(w[i], seen["grads"][i], m[i], v[i], t, 1e-2, BETAS, EPS, DECAY,
-                                          np.float32(coef), more=6, bits=state_bits)
+                                          np.float32(coef), more=6)
             _near(p, new, tol, f"parameter {i}, step {t}")
             st = opt.state[p]
             if state_bits == 32:
