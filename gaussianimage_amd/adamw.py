@@ -24,7 +24,8 @@ _CODES = torch.float8_e4m3fn
 def grad_norm(grads, max_norm=None):
     """2-norm of all ``grads`` together, and ``min(1, max_norm / (norm + 1e-6))``: two float32
     scalars on the device (``(norm, None)`` without ``max_norm``).  Float32, bfloat16 and float16
-    gradients may be mixed.  Squares are summed in double and in a fixed order."""
+    gradients may be mixed.  Squares are summed in double and in a fixed order.  A NaN among them
+    makes both results NaN, an infinity a coefficient of 0."""
     if max_norm is not None and not max_norm >= 0.0:
         raise ValueError(f"grad_norm: max_norm must be >= 0, got {max_norm}")
     limit = float("inf") if max_norm is None else float(max_norm)
@@ -267,7 +268,8 @@ class AdamW(Optimizer):
     ``state_bits``: 32, or 8 for states of two bytes per element (see ``adamw_step_8bit``;
     ``seed`` drives their rounding).  ``master_weights``: keep a float32 copy of every half
     parameter and update that.  ``max_grad_norm`` > 0: all gradients together are scaled to at
-    most that norm as they are read (``p.grad`` itself stays as it is).
+    most that norm as they are read (``p.grad`` itself stays as it is; all parameters must then be on
+    one device).
 
     ``capturable=True`` keeps the step counts in device memory, so that ``step()`` may be captured
     into a graph (after one step outside of it, which makes the states) and replayed; then ``lr``
@@ -359,9 +361,6 @@ class AdamW(Optimizer):
             if torch.is_tensor(lr) and not lr.is_cuda:
                 lr = float(lr)
             count += 1  # (in place for a tensor)
-            if not self.capturable:
-                for state in states:
-                    state["step"] = count
             kw = dict(step=count, lr=lr, betas=group["betas"], eps=group["eps"],
                       weight_decay=group["weight_decay"], clip=clip)
             if self.master_weights:
@@ -377,7 +376,15 @@ class AdamW(Optimizer):
                                 seed=(self.seed + 0x61C88647 * number) % 2 ** 32, **kw)
             else:
                 adamw_step(ps, gs, column("exp_avg"), column("exp_avg_sq"), **kw)
+            if not self.capturable:
+                for state in states:
+                    state["step"] = count
         return loss
+
+    def __getstate__(self):  # (torch's keeps the groups and the states only)
+        return {**super().__getstate__(),
+                **{k: getattr(self, k) for k in ("max_grad_norm", "state_bits", "seed",
+                                                 "master_weights", "capturable")}}
 
     def state_dict(self):
         """As torch's, with the step counts as plain numbers (this synchronises when they are in

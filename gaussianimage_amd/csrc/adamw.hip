@@ -155,8 +155,8 @@ template <> struct Elem<GI2D_F16> {
 };
 
 // NT: past the caches.  A call that touches more than the 256 MB of the last-level cache finds
-// nothing there and leaves nothing there: streamed, 200 M fp32 elements took 979 us instead of 1047,
-// 120 M with 8-bit states 327 instead of 361.  A smaller one finds its states again: 5.8 M elements
+// nothing there and leaves nothing there: streamed, 200 M fp32 elements took 979 us instead of 1047
+// (943 with four groups per lane), 120 M with 8-bit states 327 instead of 361.  A smaller one finds its states again: 5.8 M elements
 // 25.0 us through the caches, 26.8 streamed (12 M: 49 and 55, but 65 and 56 when something else ran
 // in between).  The host chooses by the size of the call, at half the cache.
 template <bool NT, typename V>
@@ -695,15 +695,12 @@ __global__ void adamw_scalars_kernel(AdamWScalars h, double beta1, double beta2,
 // order: the same bits in every run.
 #define NORM_THREADS 256
 #define NORM_TENSORS 232
-#ifndef NORM_GROUPS
+// Workgroups of a launch: 800 MB of fp32 took 135 us with 1024, 137 with 2048.
 #define NORM_GROUPS 1024
-#endif
-#ifndef NORM_ARRIVALS
-#define NORM_ARRIVALS 256
-#endif
-#ifndef NORM_SMALL_BYTES
+// Up to this size a lane loads 32 bytes at a time, through the caches (the step behind reads the
+// gradients again; 23 MB and a step 34.9 us, 36.3 with 128 bytes); beyond it 128 bytes, streamed: 800
+// MB 124 us against 139 with 64 bytes through the caches, 218 MB of bf16 38 against 44.
 #define NORM_SMALL_BYTES ((int64_t)32 << 20)
-#endif
 
 struct NormEntry {
     unsigned g, numel;
@@ -813,16 +810,45 @@ __device__ __forceinline__ void finish_norm(const double *partials, int n, float
     out[1] = c < 1.0f || c != c ? c : 1.0f;
 }
 
-// `arrived`: nullptr, or the number of workgroups that have left their partial, 0 between calls: the
-// last one to arrive finishes the norm (`before`: partials of earlier launches of this call).  The
-// order of arrival chooses who adds the partials, not the order in which they are added.
+// `arrived`: nullptr, or counters of the workgroups that have left their partial, all 0 between
+// calls: the last one to arrive finishes the norm (`before`: partials of earlier launches of this
+// call).  The order of arrival chooses who adds the partials, not the order in which they are added.
+// 16 counters, each in a line of its own, and one for the 16: atomics on one line follow each other
+// at 10 ns (2048 workgroups on one counter took 20 us more, a second launch takes 4).  Short lists
+// only: 240 k gradients 5.5 us instead of 8.0 with the second launch, which waits for the host;
+// with 1024 workgroups it is hidden, and a clipped step of 109 M elements took 231 us with it and
+// 233 without.
+#define NORM_COUNTERS 16
+#define NORM_ARRIVALS 256  // workgroups
+static_assert((NORM_COUNTERS + 1) * 32 == GI2D_GRAD_NORM_ARRIVALS, "a line each");
+
+__device__ __forceinline__ bool last_to_arrive(unsigned *arrived, int groups)
+{
+    // The partials alone pass between workgroups, and they do not go through the L2 caches (stores
+    // and loads of agent scope): once the store has been acknowledged, whoever reads a later count
+    // finds it.  A release would write back the whole L2 of the XCD.
+    __builtin_amdgcn_s_waitcnt(0);
+    const int mine = (int)blockIdx.x % NORM_COUNTERS;
+    unsigned *const counter = arrived + 32 * mine;
+    const unsigned here = (unsigned)((groups - mine + NORM_COUNTERS - 1) / NORM_COUNTERS);
+    if (__hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != here - 1u)
+        return false;
+    __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    unsigned *const all = arrived + 32 * NORM_COUNTERS;
+    const unsigned counters = (unsigned)(groups < NORM_COUNTERS ? groups : NORM_COUNTERS);
+    if (__hip_atomic_fetch_add(all, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != counters - 1u)
+        return false;
+    __hip_atomic_store(all, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return true;
+}
+
 template <int LOADS>
 __global__ __launch_bounds__(NORM_THREADS) void grad_squares_kernel(NormTable T, double *partials,
                                                                     int before, unsigned *arrived,
                                                                     float max_norm, float *out)
 {
     __shared__ double lds[NORM_THREADS / WAVE];
-    __shared__ unsigned place;
+    __shared__ bool last;
     const int lane = threadIdx.x & (WAVE - 1);
     static_assert(NORM_TENSORS > 3 * WAVE && NORM_TENSORS <= 4 * WAVE, "four ballots");
     const int f0 = T.first[lane], f1 = T.first[lane + WAVE], f2 = T.first[lane + 2 * WAVE];
@@ -845,19 +871,11 @@ __global__ __launch_bounds__(NORM_THREADS) void grad_squares_kernel(NormTable T,
     const double t = block_sum((s[0] + s[1]) + (s[2] + s[3]), lds);
     if (threadIdx.x == 0) {
         __hip_atomic_store(partials + before + blockIdx.x, t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (arrived) {
-            // The partials alone pass between workgroups, and they do not go through the L2 caches
-            // (stores and loads of agent scope): once the store has been acknowledged, whoever
-            // reads a later count finds it.  A release would write back the whole L2 of the XCD.
-            __builtin_amdgcn_s_waitcnt(0);
-            place = __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
+        if (arrived) last = last_to_arrive(arrived, T.groups);
     }
     if (!arrived) return;
     __syncthreads();
-    if (place != (unsigned)T.groups - 1u) return;
-    finish_norm(partials, before + T.groups, max_norm, out, lds);
-    if (threadIdx.x == 0) __hip_atomic_store(arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (last) finish_norm(partials, before + T.groups, max_norm, out, lds);
 }
 
 // The second launch of a call without `arrived`.
@@ -992,11 +1010,12 @@ int gi2d_adamw_step(int num_tensors, const gi2d_adamw_tensor *tensors,
     const bool on_device = hyper->step_dev || hyper->lr_dev;
     if (hyper->state_bits != 32 && hyper->state_bits != 8) return GI2D_E_INVALID;
     if ((!hyper->step_dev && hyper->step < 1) || (on_device && !hyper->scalars_dev)) return GI2D_E_INVALID;
+    if (!aligned(hyper->scalars_dev, alignof(AdamWScalars))) return GI2D_E_INVALID;
     if (!(hyper->beta1 >= 0.0 && hyper->beta1 < 1.0 && hyper->beta2 >= 0.0 && hyper->beta2 < 1.0))
         return GI2D_E_INVALID;
     const bool bits8 = hyper->state_bits == 8;
     unsigned present = 0;  // one bit per (parameter type, gradient type, masters)
-    int64_t bytes = 0;     // of memory the call touches
+    int64_t bytes = 0;     // of memory the call touches (counted up to STREAM_PAST_BYTES)
     for (int i = 0; i < num_tensors; ++i) {
         const gi2d_adamw_tensor &t = tensors[i];
         if (!type_ok(t.param_type) || !type_ok(t.grad_type) || t.numel < 0 ||
@@ -1010,8 +1029,9 @@ int gi2d_adamw_step(int num_tensors, const gi2d_adamw_tensor *tensors,
                                    t.exp_avg_sq_scale, t.master};
         for (const void *x : all)
             if (!has_48_bits(x)) return GI2D_E_INVALID;
-        bytes += t.numel * (type_size(t.param_type) + type_size(t.grad_type) + (bits8 ? 2 : 8) +
-                            (t.master ? 4 : 0));
+        if (bytes <= STREAM_PAST_BYTES)
+            bytes += t.numel * (type_size(t.param_type) + type_size(t.grad_type) + (bits8 ? 2 : 8) +
+                                (t.master ? 4 : 0));
         present |= 1u << (t.param_type * 6 + t.grad_type * 2 + (t.master ? 1 : 0));
     }
     if (!present) return GI2D_OK;
@@ -1064,7 +1084,7 @@ int gi2d_grad_norm(int num_tensors, const void *const *grads, const int64_t *num
         if (!type_ok(types[i]) || numel[i] < 0 || numel[i] > ADAMW_MAX_NUMEL ||
             (numel[i] > 0 && !grads[i]) || !has_48_bits(grads[i]))
             return GI2D_E_INVALID;
-        bytes += numel[i] * type_size(types[i]);
+        if (bytes <= NORM_SMALL_BYTES) bytes += numel[i] * type_size(types[i]);
     }
     const bool small = bytes <= NORM_SMALL_BYTES;
     const int chunk_bytes = NORM_THREADS * 16 * (small ? 2 : 8);

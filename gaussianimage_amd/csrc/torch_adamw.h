@@ -263,7 +263,7 @@ void step(const char *op, int bits, const py::object &params_, const py::object 
     for (c10::TensorImpl *t : out) written(t);
 }
 
-// The word of a stream that gi2d_grad_norm's workgroups count their arrivals in (0 between calls;
+// The words of a stream that gi2d_grad_norm's workgroups count their arrivals in (0 between calls;
 // kept for the life of the process).  nullptr while the stream is captured: a graph may be replayed
 // next to another one that was captured on the same stream.
 uint32_t *arrivals(const at::Device &device, hipStream_t stream)
@@ -278,7 +278,7 @@ uint32_t *arrivals(const at::Device &device, hipStream_t stream)
     static auto &words = *new std::map<std::pair<int, hipStream_t>, at::Tensor>();
     std::lock_guard<std::mutex> hold(lock);
     at::Tensor &t = words[{(int)device.index(), stream}];
-    if (!t.defined()) t = at::zeros({1}, at::TensorOptions().dtype(at::kInt).device(device));
+    if (!t.defined()) t = at::zeros({GI2D_GRAD_NORM_ARRIVALS}, at::TensorOptions().dtype(at::kInt).device(device));
     return reinterpret_cast<uint32_t *>(t.data_ptr<int>());
 }
 

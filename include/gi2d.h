@@ -311,7 +311,8 @@ int gi2d_adan_step(int num_tensors, float *const *params, float *const *grads,
  * parameter may have an fp32 master, which is then what is read and updated, the parameter its
  * rounding.  The gradients are not written.  One launch per 124 tensors of the
  * same types (99 with masters, 82 with 8-bit states, 70 with both); nothing is allocated and nothing is read on the host, so a call may be captured.
- * No element may appear twice among what a call writes.
+ * No element may appear twice among what a call writes.  The device of the tensors and the stream
+ * is the current one.
  * state_bits 32: exp_avg and exp_avg_sq are fp32.
  * state_bits 8: for GI2D_ADAMW_BLOCK consecutive elements one power-of-two scale and one e4m3 code
  * each: m = code * scale, sqrt(v) = code * scale.  exp_avg / exp_avg_sq hold the codes (numel
@@ -340,8 +341,8 @@ typedef struct gi2d_adamw_hyper {
     uint32_t seed; /* state_bits 8 only */
     int state_bits;
     /* for captured steps: the step count and the learning rate in device memory (either may be
-     * NULL), read when the step runs; scalars_dev: GI2D_ADAMW_SCALARS_BYTES of device memory that
-     * belong to this call until it has run */
+     * NULL), read when the step runs; scalars_dev: GI2D_ADAMW_SCALARS_BYTES of device memory, on a
+     * boundary of 32 bytes, that belong to this call until it has run */
     const int64_t *step_dev;
     const float *lr_dev;
     void *scalars_dev;
@@ -354,9 +355,11 @@ int gi2d_adamw_step(int num_tensors, const gi2d_adamw_tensor *tensors,
 /* 2-norm of all gradients together: out[0] = sqrt(sum g^2), summed in double and in a fixed order,
  * out[1] = min(1, max_norm / (out[0] + 1e-6)).  Host arrays of device pointers, element counts and
  * element types; `workspace`: gi2d_grad_norm_workspace(num_tensors) bytes of device memory that
- * belong to this call until it has run; arrived: NULL, or one word of device memory that is 0 before
- * the call and 0 again when it has run, and that no call uses meanwhile (with it the norm is
- * finished by the last workgroup instead of a second launch); out: two floats in device memory. */
+ * belong to this call until it has run; arrived: NULL, or GI2D_GRAD_NORM_ARRIVALS words of device
+ * memory (on a boundary of 128 bytes for speed) that are 0 before the call and 0 again when it has
+ * run, and that no other call uses meanwhile: with them the norm of a short list is finished by
+ * the last workgroup instead of a second launch; out: two floats in device memory. */
+#define GI2D_GRAD_NORM_ARRIVALS 544
 int64_t gi2d_grad_norm_workspace(int num_tensors);
 int gi2d_grad_norm(int num_tensors, const void *const *grads, const int64_t *numel,
                    const int *types, double max_norm, void *workspace, uint32_t *arrived, float *out,

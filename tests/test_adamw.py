@@ -194,7 +194,8 @@ def test_c_entries_refuse_without_a_device():
     assert lib.gi2d_adamw_step(1, None, hyper(), None, None) == bad
     assert lib.gi2d_adamw_step(0, None, None, None, None) == bad
     for kw in (dict(step=0), dict(state_bits=4), dict(beta1=1.0), dict(beta2=-0.1),
-               dict(beta1=float("nan")), dict(step_dev=64), dict(lr_dev=64)):
+               dict(beta1=float("nan")), dict(step_dev=64), dict(lr_dev=64),
+               dict(step_dev=64, scalars_dev=72)):
         assert lib.gi2d_adamw_step(1, table(), hyper(**kw), None, None) == bad, kw
     for kw in (dict(param=None), dict(grad=None), dict(exp_avg=None), dict(exp_avg_sq=None),
                dict(numel=-1), dict(numel=2 ** 34 + 1), dict(param_type=3), dict(grad_type=-1),
@@ -908,6 +909,38 @@ def test_state_dict_goes_on_with_the_same_bits(state_bits, capturable, tmp_path)
                 if torch.is_tensor(x) else x == y
     with pytest.raises(ValueError, match="state_bits"):
         AdamW(rs, state_bits=40 - state_bits).load_state_dict(first.state_dict())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("capturable", [False, True])
+def test_copies_of_an_optimizer(capturable):
+    import copy
+    from gaussianimage_amd.adamw import AdamW
+    ps = [torch.nn.Parameter(torch.full((n,), 0.5, device=DEV)) for n in (300, 7)]
+    opt = AdamW(ps, state_bits=8, max_grad_norm=1.0, capturable=capturable, seed=4)
+    for p in ps:
+        p.grad = torch.linspace(-1, 1, p.numel(), device=DEV)
+    opt.step()
+    other = copy.deepcopy({"opt": opt, "ps": ps})
+    qs = [p for g in other["opt"].param_groups for p in g["params"]]
+    for q, p in zip(qs, ps):
+        q.grad = p.grad.clone()
+    opt.step()
+    other["opt"].step()
+    for q, p in zip(qs, ps):
+        assert q is not p and torch.equal(q, p)
+        assert int(other["opt"].state[q]["step"]) == int(opt.state[p]["step"]) == 2
+
+
+@pytest.mark.gpu
+def test_a_failed_step_does_not_count():
+    from gaussianimage_amd.adamw import AdamW
+    p = torch.nn.Parameter(torch.zeros(8, device=DEV, dtype=torch.float64))
+    opt = AdamW([p])
+    p.grad = torch.ones_like(p)
+    with pytest.raises(ValueError, match="float32, bfloat16 or float16"):
+        opt.step()
+    assert opt.state[p]["step"] == 0
 
 
 @pytest.mark.gpu
