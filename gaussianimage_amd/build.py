@@ -78,7 +78,7 @@ def build_native(force=False, extra_flags=(), verbose=False, jobs=None):
 
 
 TORCH_OPS_SRC = os.path.join(CSRC, "torch_ops.cpp")
-TORCH_OPS_DEPS = [TORCH_OPS_SRC, os.path.join(CSRC, "torch_adamw.h"),
+TORCH_OPS_DEPS = [TORCH_OPS_SRC, os.path.join(CSRC, "torch_adamw.hpp"),
                   os.path.join(os.path.dirname(_HERE), "include", "gi2d.h")]
 TORCH_OPS_LIB = os.path.join(_HERE, "_torch_ops.so")
 

@@ -18,10 +18,11 @@
 // against 1642 (100 M the same; with 1 they vary with where the arrays lie, 5.3 to 6.0 TB/s).
 #define GROUPS32(NT) ((NT) ? 4 : 2)
 #define ADAMW_CHUNK32(NT) (GROUPS32(NT) * 4 * ADAMW_THREADS)  // elements of a workgroup
-// Blocks of 256 elements of a wave with 8-bit states: 120 M fp32 elements 311 us, 109 M bf16 177;
-// with 2 blocks 314 and 188.
-#define BLOCKS8 4
-#define ADAMW_CHUNK8 (ADAMW_THREADS / WAVE * BLOCKS8 * GI2D_ADAMW_BLOCK)
+// Blocks of 256 elements of a wave with 8-bit states.  Streamed 4: 120 M fp32 elements 311 us, 109 M
+// bf16 177; with 2 blocks 314 and 188.  Through the caches 2: 0.5 M bf16 elements 4.8 us, 10 M 22.3;
+// 4.4 and 24.1 with 1 block, 5.9 and 22.3 with 4.
+#define BLOCKS8(NT) ((NT) ? 4 : 2)
+#define ADAMW_CHUNK8(NT) (ADAMW_THREADS / WAVE * BLOCKS8(NT) * GI2D_ADAMW_BLOCK)
 #define ADAMW_MAX_NUMEL ((int64_t)1 << 34)
 #define ADAMW_MAX_CHUNKS (1 << 23)  // chunks of a launch: 256 lanes each, below 2^32 lanes
 #define STREAM_PAST_BYTES ((int64_t)128 << 20)  // (see load_vec)
@@ -565,8 +566,8 @@ __global__ __launch_bounds__(ADAMW_THREADS) void adamw_step8_kernel(
     const Factors8 f(h, clip);
     const int lane = threadIdx.x & (WAVE - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-    constexpr int OWN = BLOCKS8 * GI2D_ADAMW_BLOCK;  // elements of a wave
-    const long long block = (long long)t.chunk * (ADAMW_CHUNK8 / GI2D_ADAMW_BLOCK) + wave * BLOCKS8;
+    constexpr int BLOCKS = BLOCKS8(NT), OWN = BLOCKS * GI2D_ADAMW_BLOCK;  // elements of a wave
+    const long long block = (long long)t.chunk * (ADAMW_CHUNK8(NT) / GI2D_ADAMW_BLOCK) + wave * BLOCKS;
     const long long base = block * GI2D_ADAMW_BLOCK;
     if (base >= t.n) return;
     const unsigned n = t.n - base < OWN ? (unsigned)(t.n - base) : OWN;  // of this wave
@@ -579,14 +580,14 @@ __global__ __launch_bounds__(ADAMW_THREADS) void adamw_step8_kernel(
     unsigned char *__restrict__ v = (unsigned char *)t.v + base;
     void *__restrict__ w = MASTER ? further<GI2D_F32>(t.w, base) : p;
     float *__restrict__ sm = t.sm + block, *__restrict__ sv = t.sv + block;
-    Four<GT> gq[BLOCKS8];
-    Four<WT> wq[BLOCKS8];
-    unsigned mc[BLOCKS8], vc[BLOCKS8];
-    float km[BLOCKS8], kv[BLOCKS8];
+    Four<GT> gq[BLOCKS];
+    Four<WT> wq[BLOCKS];
+    unsigned mc[BLOCKS], vc[BLOCKS];
+    float km[BLOCKS], kv[BLOCKS];
     const bool groups = t.vec && n >= 4;  // (see adamw_step_kernel)
     if (groups) {
 #pragma unroll
-        for (int u = 0; u < BLOCKS8; ++u) {
+        for (int u = 0; u < BLOCKS; ++u) {
             const unsigned i = 4 * lane + u * GI2D_ADAMW_BLOCK;
             const bool whole = i + 4 <= n;
             gq[u].template load<NT>(g, i, whole);
@@ -596,7 +597,7 @@ __global__ __launch_bounds__(ADAMW_THREADS) void adamw_step8_kernel(
         }
     }
 #pragma unroll
-    for (int u = 0; u < BLOCKS8; ++u) {
+    for (int u = 0; u < BLOCKS; ++u) {
         km[u] = sm[u < blocks ? u : 0];
         kv[u] = sv[u < blocks ? u : 0];
         const unsigned i = 4 * lane + u * GI2D_ADAMW_BLOCK;
@@ -609,7 +610,7 @@ __global__ __launch_bounds__(ADAMW_THREADS) void adamw_step8_kernel(
     }
     int em = 0, er = 0;  // lane u: the exponents of block u
 #pragma unroll
-    for (int u = 0; u < BLOCKS8; ++u) {
+    for (int u = 0; u < BLOCKS; ++u) {
         if (u >= blocks) break;
         const unsigned i = 4 * lane + u * GI2D_ADAMW_BLOCK;
         float gx[4], wx[4];
@@ -943,7 +944,7 @@ static int adamw_run(int num_tensors, const gi2d_adamw_tensor *ts, bool stream_p
         block0 += (unsigned)((t.numel + GI2D_ADAMW_BLOCK - 1) / GI2D_ADAMW_BLOCK);
         if (t.numel == 0 || t.param_type != PT || t.grad_type != GT || (t.master != nullptr) != MASTER)
             continue;
-        const int chunk = BITS == 8 ? ADAMW_CHUNK8 : ADAMW_CHUNK32(stream_past);
+        const int chunk = BITS == 8 ? ADAMW_CHUNK8(stream_past) : ADAMW_CHUNK32(stream_past);
         const int more = (int)((t.numel + chunk - 1) / chunk);
         if (count == N || chunks + more > ADAMW_MAX_CHUNKS) {
             const int rc = flush();

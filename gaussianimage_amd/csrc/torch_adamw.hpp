@@ -1,4 +1,4 @@
-// torch_adamw.h -- gi2d_adamw_step and gi2d_grad_norm over Python lists of tensors (part of
+// torch_adamw.hpp -- gi2d_adamw_step and gi2d_grad_norm over Python lists of tensors (part of
 // torch_ops.cpp).  A list of some hundred small tensors is stepped in tens of microseconds on the
 // GPU, so the lists are read through the C API of lists, one pass, without a reference count per
 // tensor.  adamw.py holds the same calls over ctypes; both make the same checks.

@@ -503,7 +503,7 @@ at::Tensor py_rasterize_sum(const at::Tensor &xys, const at::Tensor &radii, cons
                           (int)W);
 }
 
-#include "torch_adamw.h"
+#include "torch_adamw.hpp"
 
 }  // namespace
 
