@@ -57,11 +57,33 @@ inline void need_gpu(const char *op, const at::Tensor &t)
     throw std::runtime_error(msg.str());
 }
 
+inline bool dense_layout(const at::Tensor &t)
+{
+    return t.unsafeGetTensorImpl()->key_set().has(c10::DispatchKey::Dense);
+}
+
+inline bool same(at::IntArrayRef a, at::IntArrayRef b)
+{
+    if (a.size() != b.size()) return false;
+    for (size_t i = 0; i < a.size(); ++i)
+        if (a[i] != b[i]) return false;
+    return true;
+}
+
 // `t` holds its elements in the same places as `p` does, without gaps.
 inline bool same_layout(const at::Tensor &t, const at::Tensor &p, bool p_contiguous)
 {
-    if (t.sizes() != p.sizes()) return false;
-    return p_contiguous ? t.is_contiguous() : t.strides() == p.strides();
+    if (!same(t.sizes(), p.sizes())) return false;
+    return p_contiguous ? t.is_contiguous() : same(t.strides(), p.strides());
+}
+
+// Where a tensor with elements begins (data_ptr() without what only tensors without storage need).
+inline char *start(const at::Tensor &t)
+{
+    c10::TensorImpl *impl = t.unsafeGetTensorImpl();
+    if (!impl->has_storage()) return static_cast<char *>(t.data_ptr());  // (which says why not)
+    char *base = static_cast<char *>(impl->unsafe_storage().unsafeGetStorageImpl()->mutable_data());
+    return base + (size_t)impl->storage_offset() * impl->itemsize();
 }
 
 // Set of addresses that a call writes: a tensor given twice would be updated by two workgroups at
@@ -103,7 +125,8 @@ class Written {
 
 inline void written(c10::TensorImpl *t)
 {
-    if (!t->is_inference()) t->bump_version();
+    // (a tensor made in inference mode has no version, and lacks this key)
+    if (t->key_set().has(c10::DispatchKey::ADInplaceOrView)) t->bump_version();
 }
 
 inline const at::Tensor *device_scalar(const char *op, const char *name, const py::object &o,
@@ -185,7 +208,7 @@ void step(const char *op, int bits, const py::object &params_, const py::object 
         const at::Tensor *const all[5] = {&p, &g, &mi, &vi, w};
         for (const at::Tensor *x : all)
             if (x != nullptr) {
-                if (x->layout() != at::kStrided) refuse(op, "params", i, "or what belongs to it is not strided");
+                if (!dense_layout(*x)) refuse(op, "params", i, "or what belongs to it is not strided");
                 if (x->device() != device) refuse(op, "params", i, "or what belongs to it is on another device");
             }
         t.param_type = element_type(p);
@@ -202,17 +225,17 @@ void step(const char *op, int bits, const py::object &params_, const py::object 
             refuse(op, v.name, i, state_what);
         t.numel = p.numel();
         if (t.numel > (int64_t)1 << 34) refuse(op, "params", i, "has more than 2^34 elements");
-        t.param = p.data_ptr();
-        t.grad = g.data_ptr();
-        t.exp_avg = mi.data_ptr();
-        t.exp_avg_sq = vi.data_ptr();
+        t.param = t.numel ? start(p) : nullptr;
+        t.grad = t.numel ? start(g) : nullptr;
+        t.exp_avg = t.numel ? start(mi) : nullptr;
+        t.exp_avg_sq = t.numel ? start(vi) : nullptr;
         t.exp_avg_scale = t.exp_avg_sq_scale = t.master = nullptr;
         bool fresh = t.numel == 0 || (seen.add(t.param) && seen.add(t.exp_avg) && seen.add(t.exp_avg_sq));
         if (w != nullptr) {
             if (t.param_type == GI2D_F32) refuse(op, "masters", i, "belongs to a float32 parameter");
             if (w->scalar_type() != at::kFloat || !same_layout(*w, p, contiguous))
                 refuse(op, "masters", i, "must be a float32 tensor laid out as its parameter");
-            t.master = t.numel ? w->data_ptr<float>() : nullptr;
+            t.master = t.numel ? (float *)start(*w) : nullptr;
             fresh = fresh && (t.numel == 0 || seen.add(t.master));
         }
         if (!fresh) refuse(op, "params", i, "or its state appears twice");
@@ -222,16 +245,16 @@ void step(const char *op, int bits, const py::object &params_, const py::object 
             const at::Tensor &a = *sm.at(i), &b = *sv.at(i);
             const int64_t blocks = (t.numel + GI2D_ADAMW_BLOCK - 1) / GI2D_ADAMW_BLOCK;
             for (const at::Tensor *x : {&a, &b})
-                if (x->scalar_type() != at::kFloat || x->numel() != blocks || !x->is_contiguous() ||
-                    x->device() != device)
+                if (!dense_layout(*x) || x->scalar_type() != at::kFloat || x->numel() != blocks ||
+                    !x->is_contiguous() || x->device() != device)
                     refuse(op, x == &a ? sm.name : sv.name, i,
                            "must be a contiguous float32 tensor with one element for 256 of the "
                            "parameter's, on its device");
             out.push_back(a.unsafeGetTensorImpl());
             out.push_back(b.unsafeGetTensorImpl());
             if (t.numel) {
-                t.exp_avg_scale = a.data_ptr<float>();
-                t.exp_avg_sq_scale = b.data_ptr<float>();
+                t.exp_avg_scale = (float *)start(a);
+                t.exp_avg_sq_scale = (float *)start(b);
                 if (!seen.add(t.exp_avg_scale) || !seen.add(t.exp_avg_sq_scale))
                     refuse(op, "params", i, "or its state appears twice");
             }
@@ -294,7 +317,7 @@ py::tuple grad_norm(const py::object &grads_, double max_norm)
     std::vector<int> type((size_t)n);
     for (int64_t i = 0; i < n; ++i) {
         const at::Tensor &g = *grads.at(i);
-        if (g.layout() != at::kStrided) refuse(op, "grads", i, "is not strided");
+        if (!dense_layout(g)) refuse(op, "grads", i, "is not strided");
         if (g.device() != device) refuse(op, "grads", i, "is on another device");
         type[(size_t)i] = element_type(g);
         if (type[(size_t)i] < 0) refuse(op, "grads", i, "must be float32, bfloat16 or float16");
@@ -302,7 +325,7 @@ py::tuple grad_norm(const py::object &grads_, double max_norm)
             refuse(op, "grads", i, "has gaps or overlaps in memory");
         numel[(size_t)i] = g.numel();
         if (g.numel() > (int64_t)1 << 34) refuse(op, "grads", i, "has more than 2^34 elements");
-        ptr[(size_t)i] = g.numel() ? g.data_ptr() : nullptr;
+        ptr[(size_t)i] = g.numel() ? start(g) : nullptr;
     }
     need_gpu(op, *grads.at(0));
     const c10::DeviceGuard guard(device);
