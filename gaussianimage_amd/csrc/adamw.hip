@@ -455,8 +455,8 @@ __device__ __forceinline__ float root_normal(float x)
 // codes.  What the codes are made of is rounded operation by operation, as the formulas are written
 // down: a last bit would send one value in a million to another code, 6 to 12 % away.  The step of
 // p takes the hardware's reciprocal (one unit in the last place) and fused sums, a ten-millionth of
-// the step: 10 bytes per element leave 266 cycles for 64 of them, and an instruction takes 4, before
-// the instructions and not the memory set the time.
+// the step.  With 10 bytes per element instructions count as much as memory: 109 M bf16 elements
+// took 200 us with 69 vector instructions per element, 180 (6.0 TB/s) with 62, 177 with 54.
 __device__ __forceinline__ Codes8 step8(const Factors8 &f, unsigned key, const float *g, float *p,
                                         unsigned cm, unsigned cr, float sm, float sr, unsigned block)
 {
