@@ -25,7 +25,7 @@ def grad_norm(grads, max_norm=None):
     """2-norm of all ``grads`` together, and ``min(1, max_norm / (norm + 1e-6))``: two float32
     scalars on the device (``(norm, None)`` without ``max_norm``).  Float32, bfloat16 and float16
     gradients may be mixed.  Squares are summed in double and in a fixed order.  A NaN among them
-    makes both results NaN, an infinity a coefficient of 0."""
+    makes both results NaN, an infinity a coefficient of 0 (NaN if ``max_norm`` is infinite too)."""
     if max_norm is not None and not max_norm >= 0.0:
         raise ValueError(f"grad_norm: max_norm must be >= 0, got {max_norm}")
     limit = float("inf") if max_norm is None else float(max_norm)
@@ -301,14 +301,15 @@ class AdamW(Optimizer):
             state["master"] = p.detach().to(torch.float32)
         return state
 
-    def _gradient(self, p):
-        g = p.grad
+    @staticmethod
+    def _gradient(p, g):
+        """``g`` laid out as ``p`` is (a copy when it is broadcast or has an order of its own)."""
         if not p.is_cuda:
             raise RuntimeError("gaussianimage_amd.AdamW steps parameters on an AMD GPU only "
                                "(there is no CPU fallback)")
         if g.layout != torch.strided:
             raise RuntimeError("AdamW: sparse gradients are not supported")
-        if g.stride() != p.stride():  # (an order of its own, or broadcast)
+        if g.stride() != p.stride():
             g = torch.empty_like(p, dtype=g.dtype, requires_grad=False).copy_(g)
         return g
 
@@ -323,26 +324,32 @@ class AdamW(Optimizer):
             raise RuntimeError("AdamW: only an optimizer made with capturable=True can be captured")
         # what is stepped together: the same group, device and step count
         calls, norm_grads, absent = {}, [], set()
+        capturable = self.capturable
         for k, group in enumerate(self.param_groups):
             fresh = {}  # device -> the count that new states share
+            call = last = None
             for p in group["params"]:
+                g = p.grad
                 state = self.state.get(p)
-                if p.grad is None:
-                    if state and self.capturable:
+                if g is None:
+                    if state and capturable:
                         absent.add(id(state["step"]))
                     continue
-                g = self._gradient(p)
+                if not (p.is_cuda and g.is_contiguous() and p.is_contiguous()):
+                    g = self._gradient(p, g)
+                device = p.device
                 if not state:
                     if capturing:
                         raise RuntimeError("AdamW: run one step before capturing (a captured "
                                            "step cannot make the states)")
-                    if self.capturable and p.device not in fresh:
-                        fresh[p.device] = torch.zeros(1, dtype=torch.int64, device=p.device)
-                    state = self.state[p] = self._new_state(
-                        p, fresh[p.device] if self.capturable else 0)
+                    if capturable and device not in fresh:
+                        fresh[device] = torch.zeros(1, dtype=torch.int64, device=device)
+                    state = self.state[p] = self._new_state(p, fresh[device] if capturable else 0)
                 count = state["step"]
-                key = (k, p.device, id(count) if self.capturable else count)
-                call = calls.setdefault(key, (count, [], [], []))
+                mark = (id(count) if capturable else count, device)
+                if call is None or mark != last:
+                    last = mark
+                    call = calls.setdefault((k, mark), (count, [], [], []))
                 call[1].append(p)
                 call[2].append(g)
                 call[3].append(state)
@@ -355,7 +362,7 @@ class AdamW(Optimizer):
         clip = None
         if self.max_grad_norm > 0:
             clip = grad_norm(norm_grads, self.max_grad_norm)[1]
-        for number, ((k, _, _), (count, ps, gs, states)) in enumerate(calls.items()):
+        for number, ((k, _), (count, ps, gs, states)) in enumerate(calls.items()):
             group = self.param_groups[k]
             lr = group["lr"]
             if torch.is_tensor(lr) and not lr.is_cuda:

@@ -157,9 +157,10 @@ template <> struct Elem<GI2D_F16> {
 
 // NT: past the caches.  A call that touches more than the 256 MB of the last-level cache finds
 // nothing there and leaves nothing there: streamed, 200 M fp32 elements took 979 us instead of 1047
-// (943 with four groups per lane), 120 M with 8-bit states 327 instead of 361.  A smaller one finds its states again: 5.8 M elements
-// 25.0 us through the caches, 26.8 streamed (12 M: 49 and 55, but 65 and 56 when something else ran
-// in between).  The host chooses by the size of the call, at half the cache.
+// (943 with four groups per lane), 120 M with 8-bit states 327 instead of 361.  A smaller one finds
+// its states again: 5.8 M elements 25.0 us through the caches, 26.8 streamed (12 M: 49 and 55, but
+// 65 and 56 when something else ran in between).  The host chooses by the size of the call, at half
+// the cache.
 template <bool NT, typename V>
 __device__ __forceinline__ V load_vec(const V *p)
 {
@@ -827,8 +828,8 @@ __device__ __forceinline__ bool last_to_arrive(unsigned *arrived, int groups)
 {
     // The partials alone pass between workgroups, and they do not go through the L2 caches (stores
     // and loads of agent scope): once the store has been acknowledged, whoever reads a later count
-    // finds it.  A release would write back the whole L2 of the XCD.
-    __builtin_amdgcn_s_waitcnt(0);
+    // finds it.  A release would write back the whole L2 of the XCD (with 2048 workgroups 95 us more).
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     const int mine = (int)blockIdx.x % NORM_COUNTERS;
     unsigned *const counter = arrived + 32 * mine;
     const unsigned here = (unsigned)((groups - mine + NORM_COUNTERS - 1) / NORM_COUNTERS);

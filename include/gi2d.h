@@ -310,15 +310,16 @@ int gi2d_adan_step(int num_tensors, float *const *params, float *const *grads,
  * Parameters and gradients are fp32, bf16 or fp16, each tensor its own; arithmetic is fp32.  A half
  * parameter may have an fp32 master, which is then what is read and updated, the parameter its
  * rounding.  The gradients are not written.  One launch per 124 tensors of the
- * same types (99 with masters, 82 with 8-bit states, 70 with both); nothing is allocated and nothing is read on the host, so a call may be captured.
+ * same types (99 with masters, 82 with 8-bit states, 70 with both); nothing is allocated and
+ * nothing is read on the host, so a call may be captured.
  * No element may appear twice among what a call writes.  The device of the tensors and the stream
  * is the current one.
  * state_bits 32: exp_avg and exp_avg_sq are fp32.
  * state_bits 8: for GI2D_ADAMW_BLOCK consecutive elements one power-of-two scale and one e4m3 code
  * each: m = code * scale, sqrt(v) = code * scale.  exp_avg / exp_avg_sq hold the codes (numel
- * bytes; all-zero codes are a fresh state whatever the scales), the scales are fp32, one for each
- * block.  The codes are rounded at random with the mean kept, by a hash of (seed, step, block,
- * element): the same call gives the same bits.  Infinities and NaN become the NaN code. */
+ * bytes; all-zero codes are a fresh state whatever finite scales stand beside them), the scales are
+ * fp32, one for each block.  The codes are rounded at random with the mean kept, by a hash of (seed,
+ * step, block, element): the same call gives the same bits.  Infinities and NaN become the NaN code. */
 #define GI2D_F32 0
 #define GI2D_BF16 1
 #define GI2D_F16 2

@@ -933,6 +933,34 @@ def test_copies_of_an_optimizer(capturable):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("state_bits", [32, 8])
+def test_scalars_strides_and_inference_tensors(state_bits, binding):
+    """A parameter of no dimensions, one in another order with a gradient in a third, and states
+    made in inference mode, against contiguous copies of the same."""
+    from gaussianimage_amd.adamw import AdamW, adamw_step
+    gen = torch.Generator().manual_seed(2)
+    x, y = torch.randn(9, 70, generator=gen), torch.randn(9, 70, generator=gen)
+    a = [torch.nn.Parameter(torch.tensor(0.5, device=DEV)),
+         torch.nn.Parameter(x.t().contiguous().to(DEV).t())]
+    b = [torch.nn.Parameter(torch.full((1,), 0.5, device=DEV)),
+         torch.nn.Parameter(x.t().contiguous().to(DEV))]
+    assert not a[1].is_contiguous()
+    a[0].grad, b[0].grad = torch.tensor(0.25, device=DEV), torch.full((1,), 0.25, device=DEV)
+    a[1].grad, b[1].grad = y.to(DEV), y.t().contiguous().to(DEV)
+    for ps in (a, b):
+        opt = AdamW(ps, state_bits=state_bits, seed=1)
+        for _ in range(3):
+            opt.step()
+    assert torch.equal(a[0].reshape(1), b[0]) and torch.equal(a[1].t(), b[1])
+    with torch.inference_mode():
+        p, g, m, v = (torch.full((300,), s, device=DEV) for s in (0.5, 0.25, 0.0, 0.0))
+        adamw_step([p], [g], [m], [v], step=1)
+    q = torch.full((300,), 0.5, device=DEV)
+    adamw_step([q], [g], [torch.zeros(300, device=DEV)], [torch.zeros(300, device=DEV)], step=1)
+    assert torch.equal(p, q)
+
+
+@pytest.mark.gpu
 def test_a_failed_step_does_not_count():
     from gaussianimage_amd.adamw import AdamW
     p = torch.nn.Parameter(torch.zeros(8, device=DEV, dtype=torch.float64))
