@@ -47,7 +47,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.
     float32 tensor of one element on the device, both read when the step runs (for captured
     steps).  ``clip``: a device scalar, ``grad_norm``'s second result.  Gradients are not written.
 
-    Every tensor must be dense, and a parameter's gradient and states laid out as it is.
+    Every tensor must be dense, and a parameter's gradient and states laid out as it is.  Nothing
+    that the call writes may overlap anything else of it (a tensor given twice is refused).
     """
     (ops._C if ops._USE_C else _ctypes_binding).adamw_step(
         "adamw_step", 32, params, grads, exp_avgs, exp_avg_sqs, None, None, masters, step, lr,
@@ -158,8 +159,8 @@ class _ctypes_binding:
 
             for x in (p, grads[i], exp_avgs[i], exp_avg_sqs[i], w):
                 if x is not None:
-                    if x.layout != torch.strided:
-                        refuse("params", "or what belongs to it is not strided")
+                    if x.layout != torch.strided or x.is_neg():
+                        refuse("params", "or what belongs to it is not strided or a negated view")
                     if x.device != device:
                         refuse("params", "or what belongs to it is on another device")
             for name, x in (("params", p), ("grads", grads[i])):
@@ -237,8 +238,8 @@ class _ctypes_binding:
         for i, g in enumerate(grads):
             if not torch.is_tensor(g):
                 raise TypeError(f"grads[{i}] is not a tensor")
-            if g.layout != torch.strided:
-                raise ValueError(f"grad_norm: grads[{i}] is not strided")
+            if g.layout != torch.strided or g.is_neg():
+                raise ValueError(f"grad_norm: grads[{i}] is not strided or a negated view")
             if g.device != grads[0].device:
                 raise ValueError(f"grad_norm: grads[{i}] is on another device")
             if g.dtype not in _TYPES:

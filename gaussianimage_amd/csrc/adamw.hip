@@ -1015,6 +1015,10 @@ int gi2d_adamw_step(int num_tensors, const gi2d_adamw_tensor *tensors,
     if (!aligned(hyper->scalars_dev, alignof(AdamWScalars))) return GI2D_E_INVALID;
     if (!(hyper->beta1 >= 0.0 && hyper->beta1 < 1.0 && hyper->beta2 >= 0.0 && hyper->beta2 < 1.0))
         return GI2D_E_INVALID;
+    if (!(hyper->eps >= 0.0) || !(hyper->weight_decay >= 0.0) || (!hyper->lr_dev && !(hyper->lr >= 0.0)))
+        return GI2D_E_INVALID;
+    if (!aligned(hyper->step_dev, 8) || !aligned(hyper->lr_dev, 4) || !aligned(clip_dev, 4))
+        return GI2D_E_INVALID;
     const bool bits8 = hyper->state_bits == 8;
     unsigned present = 0;  // one bit per (parameter type, gradient type, masters)
     int64_t bytes = 0;     // of memory the call touches (counted up to STREAM_PAST_BYTES)
@@ -1031,6 +1035,11 @@ int gi2d_adamw_step(int num_tensors, const gi2d_adamw_tensor *tensors,
                                    t.exp_avg_sq_scale, t.master};
         for (const void *x : all)
             if (!has_48_bits(x)) return GI2D_E_INVALID;
+        const int state = bits8 ? 1 : 4;
+        if (!aligned(t.param, type_size(t.param_type)) || !aligned(t.grad, type_size(t.grad_type)) ||
+            !aligned(t.exp_avg, state) || !aligned(t.exp_avg_sq, state) || !aligned(t.master, 4) ||
+            (bits8 && !(aligned(t.exp_avg_scale, 4) && aligned(t.exp_avg_sq_scale, 4))))
+            return GI2D_E_INVALID;
         if (bytes <= STREAM_PAST_BYTES)
             bytes += t.numel * (type_size(t.param_type) + type_size(t.grad_type) + (bits8 ? 2 : 8) +
                                 (t.master ? 4 : 0));
@@ -1081,10 +1090,12 @@ int gi2d_grad_norm(int num_tensors, const void *const *grads, const int64_t *num
 {
     if (num_tensors < 0 || !out || !workspace || !(max_norm >= 0.0)) return GI2D_E_INVALID;
     if (num_tensors > 0 && (!grads || !numel || !types)) return GI2D_E_INVALID;
+    if (!aligned(workspace, 8) || !aligned(arrived, 4) || !aligned(out, 4)) return GI2D_E_INVALID;
     int64_t bytes = 0;
     for (int i = 0; i < num_tensors; ++i) {
         if (!type_ok(types[i]) || numel[i] < 0 || numel[i] > ADAMW_MAX_NUMEL ||
-            (numel[i] > 0 && !grads[i]) || !has_48_bits(grads[i]))
+            (numel[i] > 0 && !grads[i]) || !has_48_bits(grads[i]) ||
+            !aligned(grads[i], type_size(types[i])))
             return GI2D_E_INVALID;
         if (bytes <= NORM_SMALL_BYTES) bytes += numel[i] * type_size(types[i]);
     }

@@ -57,9 +57,11 @@ inline void need_gpu(const char *op, const at::Tensor &t)
     throw std::runtime_error(msg.str());
 }
 
+// (a negated view -- z.conj().imag is one -- holds other values in memory than it stands for)
 inline bool dense_layout(const at::Tensor &t)
 {
-    return t.unsafeGetTensorImpl()->key_set().has(c10::DispatchKey::Dense);
+    const c10::DispatchKeySet keys = t.unsafeGetTensorImpl()->key_set();
+    return keys.has(c10::DispatchKey::Dense) && !keys.has(c10::DispatchKey::Negative);
 }
 
 inline bool same(at::IntArrayRef a, at::IntArrayRef b)
@@ -158,6 +160,8 @@ void step(const char *op, int bits, const py::object &params_, const py::object 
         h.lr = lr_.cast<double>();
         if (!(h.lr >= 0.0)) refuse_value(op, "lr", ">= 0", h.lr);
     }
+    // (before anything is gathered: a count with an __index__ of its own may run any Python code)
+    const int64_t count = THPVariable_Check(step_.ptr()) ? 1 : step_.cast<int64_t>();
     for (double b : {betas.first, betas.second})
         if (!(b >= 0.0 && b < 1.0)) refuse_value(op, "betas", "in [0, 1)", b);
     if (!(eps >= 0.0)) refuse_value(op, "eps", ">= 0", eps);
@@ -169,7 +173,7 @@ void step(const char *op, int bits, const py::object &params_, const py::object 
     h.weight_decay = weight_decay;
     h.seed = (uint32_t)seed;
     h.state_bits = bits;
-    h.step = 1;
+    h.step = count;
     h.step_dev = nullptr;
     h.lr_dev = nullptr;
     h.scalars_dev = nullptr;
@@ -208,7 +212,7 @@ void step(const char *op, int bits, const py::object &params_, const py::object 
         const at::Tensor *const all[5] = {&p, &g, &mi, &vi, w};
         for (const at::Tensor *x : all)
             if (x != nullptr) {
-                if (!dense_layout(*x)) refuse(op, "params", i, "or what belongs to it is not strided");
+                if (!dense_layout(*x)) refuse(op, "params", i, "or what belongs to it is not strided or a negated view");
                 if (x->device() != device) refuse(op, "params", i, "or what belongs to it is on another device");
             }
         t.param_type = element_type(p);
@@ -264,8 +268,6 @@ void step(const char *op, int bits, const py::object &params_, const py::object 
     const c10::DeviceGuard guard(device);
     if (THPVariable_Check(step_.ptr()))
         h.step_dev = device_scalar(op, "step", step_, at::kLong, device)->data_ptr<int64_t>();
-    else
-        h.step = step_.cast<int64_t>();
     if (h.step < 1) throw py::value_error(std::string(op) + ": step counts from 1");
     if (THPVariable_Check(lr_.ptr()))
         h.lr_dev = device_scalar(op, "lr", lr_, at::kFloat, device)->data_ptr<float>();
@@ -317,7 +319,7 @@ py::tuple grad_norm(const py::object &grads_, double max_norm)
     std::vector<int> type((size_t)n);
     for (int64_t i = 0; i < n; ++i) {
         const at::Tensor &g = *grads.at(i);
-        if (!dense_layout(g)) refuse(op, "grads", i, "is not strided");
+        if (!dense_layout(g)) refuse(op, "grads", i, "is not strided or a negated view");
         if (g.device() != device) refuse(op, "grads", i, "is on another device");
         type[(size_t)i] = element_type(g);
         if (type[(size_t)i] < 0) refuse(op, "grads", i, "must be float32, bfloat16 or float16");

@@ -162,6 +162,72 @@ def test_refused_tensors(binding):
     step([], [], [], [])                             # nothing to do is no error
 
 
+def test_negated_views_are_refused(binding):
+    """``z.conj().imag`` is a float32 tensor whose memory holds the negative of its values."""
+    from gaussianimage_amd.adamw import adamw_step, grad_norm
+    neg = torch.zeros(1, dtype=torch.complex64).conj().imag
+    assert neg.is_neg() and neg.is_contiguous()
+    for wrong in range(4):
+        lists = [[torch.zeros(1)] for _ in range(4)]
+        lists[wrong] = [neg]
+        with pytest.raises(ValueError, match="negated"):
+            adamw_step(*lists, step=1)
+    with pytest.raises(ValueError, match="negated"):
+        grad_norm([neg])
+
+
+def test_a_count_that_runs_python_code(binding):
+    """A step count whose ``__index__`` makes another call: that call's checks do not disturb the
+    outer one's."""
+    from gaussianimage_amd.adamw import adamw_step
+    asked = []
+
+    class Count:
+        def __index__(self):
+            with pytest.raises(ValueError, match="twice"):
+                adamw_step(*[[torch.zeros(5)] * 2 for _ in range(4)], step=1)
+            asked.append(1)
+            return 0
+
+        __int__ = __index__
+
+    p, g, m, v = _cpu()
+    with pytest.raises((ValueError, RuntimeError), match="counts from 1|no CPU fallback"):
+        adamw_step(p, g, m, v, step=Count())
+
+
+def test_c_entry_refuses_hyperparameters_and_misaligned_elements():
+    from gaussianimage_amd import _lib
+
+    def call(tensor, **kw):
+        t = (_lib.AdamWTensor * 1)()
+        for k, x in {**dict(param=64, grad=64, exp_avg=64, exp_avg_sq=64, numel=4), **tensor}.items():
+            setattr(t[0], k, x)
+        h = _lib.AdamWHyper(**{**dict(lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, step=1,
+                                      state_bits=32), **kw})
+        return _lib.lib.gi2d_adamw_step(1, t, ctypes.byref(h), None, None)
+
+    for name in ("lr", "eps", "weight_decay"):
+        for x in (-1e-3, float("nan")):
+            assert call({}, **{name: x}) == _lib.GI2D_E_INVALID, (name, x)
+    for tensor in (dict(param=66), dict(grad=65), dict(param=65, param_type=1),
+                   dict(grad=65, grad_type=2), dict(exp_avg=66), dict(exp_avg_sq=65),
+                   dict(param_type=1, master=66)):
+        assert call(tensor) == _lib.GI2D_E_INVALID, tensor
+    for scale in ("exp_avg_scale", "exp_avg_sq_scale"):
+        tensor = {"exp_avg_scale": 64, "exp_avg_sq_scale": 64, scale: 66}
+        assert call(tensor, state_bits=8) == _lib.GI2D_E_INVALID, scale
+    one, size = (ctypes.c_void_p * 1)(66), (ctypes.c_int64 * 1)(4)
+    f32 = (ctypes.c_int * 1)(0)
+    assert _lib.lib.gi2d_grad_norm(1, one, size, f32, 1.0, 64, None, 64, None) == _lib.GI2D_E_INVALID
+    one[0] = 64
+    for work, arrived, out in ((68, None, 64), (64, 66, 64), (64, None, 66)):
+        assert _lib.lib.gi2d_grad_norm(1, one, size, f32, 1.0, work, arrived, out,
+                                       None) == _lib.GI2D_E_INVALID
+    for kw in (dict(step_dev=68, scalars_dev=64), dict(lr_dev=66, scalars_dev=64)):
+        assert call({}, **kw) == _lib.GI2D_E_INVALID, kw
+
+
 def test_optimizer_refuses_cpu_parameters():
     from gaussianimage_amd.adamw import AdamW
     p = [torch.nn.Parameter(torch.zeros(3))]
